@@ -268,6 +268,88 @@ WELVET_API welvet_status welvet_b200_decode_attention_static(const welvet_b200_m
                                                              const int32_t* ctx_len, void* out, int32_t ldo,
                                                              void* stream);
 
+/* ---- q/k norms and the E4M3 KV cache (no counterpart in the reference) ----
+ * Device buffers, asynchronous on `stream`; nothing is allocated after the first
+ * call on a device. Code 1 for invalid arguments, 2 for what is not built. Device
+ * faults of the data (a position past the RoPE table, a page outside the pool) leave
+ * the row or block out and are reported by welvet_b200_device_check.
+ *
+ * RoPE table: (cos, sin) of pos / theta^(2i/head_dim), [max_pos][head_dim/2][2] FP32,
+ * computed in FP64, the table the layer uses (shaders/ops_mha.metal:14-29). */
+WELVET_API welvet_status welvet_b200_rope_table(int32_t max_pos, int32_t head_dim, double theta, float* table,
+                                                void* stream);
+
+/* RMS norm of every query and key head and the position rotation in one pass:
+ * y = R(pos) (gamma * x / sqrt(mean(x^2) + eps)) for each head of head_dim values
+ * (even, at most 512). q holds tokens rows of heads * head_dim values, ldq apart
+ * (likewise k with kv_heads; kv_heads 0 and k NULL: queries only); outputs may be the
+ * inputs. q_gamma / k_gamma [head_dim] FP32; NULL leaves that side unnormalised. rope
+ * NULL: no rotation; positions [tokens], or NULL for the token index, modulo pos_mod
+ * when that is positive. Values are BF16 when io_bf16, else FP32; sums are FP32.
+ * eps <= 0 selects 1e-6. */
+WELVET_API welvet_status welvet_b200_qk_norm_rope_forward(
+    int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, double eps, const float* q_gamma,
+    const float* k_gamma, const float* rope, int32_t max_pos, const int32_t* positions, int32_t pos_mod,
+    const void* q, int64_t ldq, const void* k, int64_t ldk, void* q_out, int64_t ldq_out, void* k_out,
+    int64_t ldk_out, int32_t io_bf16, void* stream);
+/* Its gradient: from the forward's inputs q, k and the gradients dq_out, dk_out of its
+ * outputs, dq and dk (may be dq_out / dk_out) and the sums over all rows dq_gamma,
+ * dk_gamma [head_dim] FP32 (overwritten; NULL: not wanted). workspace: device memory
+ * of welvet_b200_qk_norm_rope_workspace(head_dim) bytes, 16-byte aligned, used by one
+ * call at a time. The same inputs give the same bits. */
+WELVET_API int64_t welvet_b200_qk_norm_rope_workspace(int32_t head_dim);
+WELVET_API welvet_status welvet_b200_qk_norm_rope_backward(
+    int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, double eps, const float* q_gamma,
+    const float* k_gamma, const float* rope, int32_t max_pos, const int32_t* positions, int32_t pos_mod,
+    const void* q, int64_t ldq, const void* k, int64_t ldk, const void* dq_out, int64_t lddq_out,
+    const void* dk_out, int64_t lddk_out, void* dq, int64_t lddq, void* dk, int64_t lddk, float* dq_gamma,
+    float* dk_gamma, void* workspace, int32_t io_bf16, void* stream);
+
+/* A paged cache in E4M3, 64 tokens to a page, one FP32 scale for each block of 16
+ * tokens of a KV head: value = code * scale. All pointers are device memory of the
+ * caller (codes 16-byte aligned for the tensor-core kernel).
+ *   k, v            codes [pages][kv_heads][64][head_dim]
+ *   k_scale, v_scale  [pages][kv_heads][4], positive; append writes powers of two
+ *   block_table     [batch][max_pages] page ids; entry j holds tokens [64j, 64j+64)
+ *   ctx_len         [batch] tokens of each sequence INCLUDING the new ones of the call
+ * head_dim even, at most 256. */
+#define WELVET_B200_KV8_PAGE 64
+#define WELVET_B200_KV8_BLOCK 16
+typedef struct welvet_b200_kv8_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* block_table;
+  const int32_t* ctx_len;
+  int32_t batch, pages, max_pages, kv_heads, head_dim;
+} welvet_b200_kv8_cache;
+
+/* Appends the new tokens of every sequence: BF16 rows b * seq + t of k and v
+ * (kv_heads * head_dim values, ldk / ldv apart), t < n_b = seq_lens[b] (device; NULL:
+ * seq), to positions ctx_len[b] - n_b + t. rope (not NULL) rotates the keys on the way.
+ * A block's scale is the smallest power of two s >= 2^-64 with amax <= 448 s; a block
+ * that already holds tokens keeps the larger of its scale and that, and its held codes
+ * are rewritten to it. A value that is not finite gives its block a NaN scale: the
+ * block reads as NaN until a later append begins it anew. */
+WELVET_API welvet_status welvet_b200_kv8_append(const welvet_b200_kv8_cache* cache, int32_t seq,
+                                                const int32_t* seq_lens, const void* k, int32_t ldk,
+                                                const void* v, int32_t ldv, const float* rope,
+                                                int32_t max_pos, void* stream);
+
+/* Attention of the new tokens over the cache (after the append): query row b * seq + t,
+ * t < n_b, at position p = ctx_len[b] - n_b + t sees the keys at positions <= p (mask 1)
+ * and > p - window (mask 3 with window_causal; window 0 = max_seq_len as in the layer).
+ * cfg: num_heads, num_kv_heads, head_dim, scale_override, mask, window, ALiBi (pos 2 or
+ * 3), head shard, precision 1; q and out are BF16 rows, ldq / ldo apart. Rows that see
+ * nothing (t >= n_b, an empty sequence) are zero. max_ctx bounds ctx_len (it sizes the
+ * split of long contexts, not the result's meaning). Code 2 for sigmoid scores, other
+ * masks and FP32 layers. */
+WELVET_API welvet_status welvet_b200_kv8_attention(const welvet_b200_mha_config* cfg,
+                                                   const welvet_b200_kv8_cache* cache, int32_t seq,
+                                                   const int32_t* seq_lens, int32_t max_ctx, const void* q,
+                                                   int32_t ldq, void* out, int32_t ldo, void* stream);
+
 /* ---- transformer-block forwards around the MHA (extension; the reference's
  * one-shot entries are in welvet_c.h) ----
  * Resident SwiGLU feed-forward (src/layers/swiglu/swiglu.cpp:93-143): Gate/Up

@@ -19,6 +19,8 @@ enum : uint32_t {
   kErrWaitAccEmpty = 4,
   kErrWaitOther = 5,
   kErrPeerWait = 6,   // a peer rank's data did not arrive (peer-memory all-reduce)
+  kErrRopePos = 0x100,  // token position outside the RoPE table
+  kErrKvPage = 0x101,   // block table names a page outside the pool, or ends before the context
 };
 
 // --------------------------------------------------------------------- GEMM
@@ -289,6 +291,83 @@ cudaError_t attn_decode_tc(const DecodeArgs& a, int splits, cudaStream_t s);
 // Pool layout: [page][kv_head][kPageTokens][head_dim]; slot = page*kPageTokens + row.
 cudaError_t kv_append(const void* k, const void* v, int ld, int rows, int kd, int head_dim,
                       int is_bf16, const int* slot, void* k_pool, void* v_pool, cudaStream_t s);
+
+// ---- per-head q/k norm with the position rotation (qk_norm.cu)
+constexpr int kQkNormMaxHeadDim = 512;
+constexpr int kQkNormParts = 592;  // most rows of the gamma-gradient partials (4 CTAs per SM)
+struct QkNormArgs {
+  int64_t tokens = 0;
+  int heads = 0, kv_heads = 0, head_dim = 0;  // head_dim even, at most kQkNormMaxHeadDim
+  int is_bf16 = 1;
+  float eps = 1e-6f;
+  const float* q_gamma = nullptr;  // [head_dim]; null: that side is not normalised
+  const float* k_gamma = nullptr;
+  const float2* rope = nullptr;    // [max_pos, head_dim / 2] (cos, sin); null: no rotation
+  int max_pos = 0;
+  const int* positions = nullptr;  // [tokens]; null: token index, modulo pos_mod when > 0
+  int pos_mod = 0;
+  // rows of one token: heads * head_dim values at q + t * ldq, kv_heads * head_dim at k + t * ldk
+  const void* q = nullptr;
+  const void* k = nullptr;
+  int64_t ldq = 0, ldk = 0;
+  void* q_out = nullptr;           // forward: outputs (may be q / k); backward: dq, dk
+  void* k_out = nullptr;
+  int64_t ldqo = 0, ldko = 0;
+  // backward only: gradients of the forward's outputs, and of the gammas (may be null)
+  const void* dq_out = nullptr;
+  const void* dk_out = nullptr;
+  int64_t lddqo = 0, lddko = 0;
+  float* dq_gamma = nullptr;
+  float* dk_gamma = nullptr;
+  float* partial = nullptr;        // qk_norm_workspace_bytes(head_dim)
+  int part_q = 0;                  // set by qk_norm_backward
+  uint32_t* err = nullptr;
+  int sm_count = 148;
+};
+size_t qk_norm_workspace_bytes(int head_dim);
+cudaError_t qk_norm_forward(const QkNormArgs& a, cudaStream_t s);
+cudaError_t qk_norm_backward(const QkNormArgs& a, cudaStream_t s);  // two launches
+
+// ---- paged KV cache in E4M3 with a scale per block of 16 tokens (kv8.cu)
+constexpr int kKv8Page = 64, kKv8Block = 16, kKv8Subs = kKv8Page / kKv8Block;
+constexpr int kKv8MaxHeadDim = 256;
+struct Kv8Cache {
+  void* k = nullptr;          // E4M3 codes [pages][kv_heads][64][head_dim]
+  void* v = nullptr;
+  float* k_scale = nullptr;   // [pages][kv_heads][4]
+  float* v_scale = nullptr;
+  const int* block_table = nullptr;  // [batch][max_pages]
+  const int* ctx_len = nullptr;      // [batch] tokens, the new ones included
+  int pages = 0, max_pages = 0, kv_heads = 0, head_dim = 0;
+};
+struct Kv8AppendArgs {
+  Kv8Cache c;
+  int batch = 0, seq = 0;
+  const int* seq_lens = nullptr;  // [batch] new tokens (at most seq); null: seq
+  const void* k = nullptr;        // BF16 rows b * seq + t, kv_heads * head_dim values each
+  const void* v = nullptr;
+  int ldk = 0, ldv = 0;
+  const float2* rope = nullptr;   // [max_pos, head_dim / 2]; null: keys are stored as given
+  int max_pos = 0;
+  uint32_t* err = nullptr;
+  int sm_count = 148;
+};
+cudaError_t kv8_append(const Kv8AppendArgs& a, cudaStream_t s);
+struct Kv8AttnArgs {
+  Kv8Cache c;
+  int batch = 0, seq = 0, heads = 0;
+  const int* seq_lens = nullptr;
+  int max_ctx = 0;                // upper bound of ctx_len (sizes the splits only)
+  const void* q = nullptr;        // BF16 rows b * seq + t, heads * head_dim values each
+  void* out = nullptr;
+  int ldq = 0, ldo = 0;
+  int window = 0;                 // > 0: keys (pos - window, pos]
+  int alibi = 0, head_base = 0, total_heads = 0;
+  float scale = 0.f;
+  uint32_t* err = nullptr;
+  int sm_count = 148;
+};
+cudaError_t kv8_attention(const Kv8AttnArgs& a, cudaStream_t s);
 
 // ---- transformer-block kernels (block.cu)
 struct NormArgs {

@@ -1,0 +1,198 @@
+// The paged KV cache in E4M3: appending tokens, and attention over it for every shape
+// the tensor-core kernel (kv8_attn.cu) does not take.
+//
+// Pools hold pages of 64 tokens, codes [page][kv_head][64][head_dim], and one scale
+// for each block of 16 tokens, [page][kv_head][4]; a value is code * scale. A scale is
+// the smallest power of two s >= 2^-64 with amax / s <= 448, so dividing by it and
+// changing it later are exact as long as the code stays normal: a block that gains
+// tokens with larger values takes the larger scale and its held codes are rewritten.
+// (A scale that is not a power of two would round the held codes once more each time.)
+// Per-token accuracy is that of E4M3, a relative 2^-4 for every value above 2^-14 of
+// the block's largest. A block that is given a value which is not finite gets a NaN
+// scale and reads as NaN until it is begun anew; its codes stay finite, so that a
+// masked token never reaches an output through 0 * NaN.
+// ctx_len[b] counts the new tokens: those of sequence b are at positions
+// [ctx_len - n_b, ctx_len), n_b = seq_lens ? seq_lens[b] : seq.
+// No reference counterpart (it has no KV cache).
+#include "kv8.cuh"
+
+#include <algorithm>
+
+namespace wv {
+namespace {
+
+WV_DEV float block_max(float v, float* tmp) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();  // tmp may still be read by the previous call
+  if (lane_id() == 0) tmp[warp_id()] = v;
+  __syncthreads();
+  v = tmp[0];
+  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v = fmaxf(v, tmp[w]);
+  return v;
+}
+
+// ------------------------------------------------------------------- append
+// One CTA per (block of a sequence, KV head, K or V): any even head_dim and stride.
+// Rotated keys are computed twice (once for the maximum), with the products and the
+// sum rounded one by one so that a key is the same code on every path.
+__global__ void __launch_bounds__(128) kv8_append_kernel(const Kv8AppendArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float tmp[4];
+  const int b = blockIdx.z, hd = a.c.head_dim, half = hd / 2;
+  const bool is_v = (blockIdx.y & 1) != 0;
+  const int kh = (int)(blockIdx.y >> 1);
+  const int n = kv8_new(a.seq_lens, b, a.seq), ctx = a.c.ctx_len[b], start = ctx - n;
+  const int first = max(start, 0);  // new tokens before position 0 do not exist
+  const int blk = first / kKv8Block + (int)blockIdx.x;
+  const int p0 = blk * kKv8Block, lo = max(first, p0), hi = min(ctx, p0 + kKv8Block);
+  if (lo >= hi) return;
+  const int page = kv8_page(a.c, b, blk / kKv8Subs, a.err);
+  if (page < 0) return;
+  const size_t ph = (size_t)page * a.c.kv_heads + kh;
+  uint8_t* codes = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + (ph * kKv8Page + p0 % kKv8Page) * hd;
+  float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + ph * kKv8Subs + blk % kKv8Subs;
+  const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(is_v ? a.v : a.k) + (size_t)kh * hd;
+  const int ld = is_v ? a.ldv : a.ldk;
+
+  auto pair = [&](int idx) -> float2 {  // values i and i + half of token lo + idx / half
+    const int p = lo + idx / half, i = idx % half;
+    const __nv_bfloat16* x = src + ((size_t)b * a.seq + (p - start)) * ld;
+    const float u = __bfloat162float(x[i]), w = __bfloat162float(x[half + i]);
+    if (is_v || !a.rope) return make_float2(u, w);
+    if (p >= a.max_pos) {
+      if (a.err) atomicCAS(a.err, 0u, kErrRopePos);
+      return make_float2(u, w);
+    }
+    const float2 c = a.rope[(size_t)p * half + i];
+    return make_float2(__fsub_rn(__fmul_rn(u, c.x), __fmul_rn(w, c.y)), __fadd_rn(__fmul_rn(u, c.y), __fmul_rn(w, c.x)));
+  };
+  float amax = 0.f;
+  for (int idx = threadIdx.x; idx < (hi - lo) * half; idx += blockDim.x) {
+    const float2 x = pair(idx);
+    const float m = fmaxf(fabsf(x.x), fabsf(x.y));
+    amax = fmaxf(amax, x.x - x.x == 0.f && x.y - x.y == 0.f ? m : INFINITY);  // NaN counts as infinite
+  }
+  amax = block_max(amax, tmp);
+  const float s_old = lo > p0 ? *scale : 0.f;
+  const bool poison = amax == INFINITY || s_old != s_old;
+  const float s = poison ? __uint_as_float(0x7fc00000u) : fmaxf(kv8_scale(amax), s_old);
+  for (int idx = threadIdx.x; idx < (hi - lo) * half; idx += blockDim.x) {
+    const float2 x = poison ? make_float2(0.f, 0.f) : pair(idx);
+    const uint32_t c = poison ? 0u : e4m3x2(x.x / s, x.y / s);
+    uint8_t* row = codes + (size_t)(lo - p0 + idx / half) * hd + idx % half;
+    row[0] = (uint8_t)c;
+    row[half] = (uint8_t)(c >> 8);
+  }
+  if (lo > p0 && !poison && s != s_old)
+    for (int i = threadIdx.x; i < (lo - p0) * hd; i += blockDim.x)
+      codes[i] = (uint8_t)e4m3x2(e4m3_value(codes[i]) * s_old / s, 0.f);
+  __syncthreads();  // every thread has read the old scale
+  if (threadIdx.x == 0) *scale = s;
+}
+
+// --------------------------------------------------------- attention, any shape
+constexpr int kGenWarps = 4;
+
+// One CTA per (query row, head): warp w takes the 32-key groups w, w + 4, ... of the
+// row's keys, a lane per key for the scores and a lane per dimension for the values,
+// with a running maximum and sum; the warps merge in shared memory, in warp order.
+template <bool ALIBI>
+__global__ void __launch_bounds__(kGenWarps * 32) kv8_attn_rows_kernel(const Kv8AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kDims = kKv8MaxHeadDim / 32;
+  __shared__ float qs[kKv8MaxHeadDim];
+  __shared__ float mw[kGenWarps], lw[kGenWarps], ow[kGenWarps][kKv8MaxHeadDim];
+  const int hd = a.c.head_dim, warp = (int)warp_id(), lane = (int)lane_id();
+  const int h = blockIdx.x % a.heads, t = blockIdx.x / a.heads, b = blockIdx.z;
+  const int kh = h / (a.heads / a.c.kv_heads);
+  const int n = kv8_new(a.seq_lens, b, a.seq), ctx = a.c.ctx_len[b];
+  const int qpos = ctx - n + t;
+  const size_t row = (size_t)b * a.seq + t;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row * a.ldo + (size_t)h * hd;
+  if (t >= n || qpos < 0) {  // no such token: a row that sees nothing
+    for (int d = threadIdx.x; d < hd; d += blockDim.x) out[d] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + row * a.ldq + (size_t)h * hd;
+  for (int d = threadIdx.x; d < hd; d += blockDim.x) qs[d] = __bfloat162float(q[d]);
+  __syncthreads();
+  const int k1 = qpos + 1, k0 = a.window > 0 ? max(0, k1 - a.window) : 0;
+  const float sl = a.scale * 1.4426950408889634f;
+  const float slope = ALIBI ? exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * 1.4426950408889634f : 0.f;
+  float m = -INFINITY, l = 0.f, o[kDims] = {};
+  for (int g = k0 / 32 + warp; g * 32 < k1; g += kGenWarps) {
+    const int page = kv8_page(a.c, b, g * 32 / kKv8Page, a.err);
+    if (page < 0) continue;
+    const size_t ph = (size_t)page * a.c.kv_heads + kh;
+    const int key = g * 32 + lane, slot = key % kKv8Page;
+    const bool on = key >= k0 && key < k1;
+    const uint8_t* kr = static_cast<const uint8_t*>(a.c.k) + (ph * kKv8Page + slot) * hd;
+    float x = -INFINITY;
+    if (on) {
+      float s = 0.f;
+      for (int d = 0; d < hd; ++d) s += qs[d] * e4m3_value(kr[d]);
+      x = s * a.c.k_scale[ph * kKv8Subs + slot / kKv8Block] * sl;
+      if (ALIBI) x -= slope * (float)(qpos - key);
+    }
+    float mx = x;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    const float mnew = fmaxf(m, mx);
+    const float corr = m == -INFINITY ? 0.f : exp2f(m - mnew);
+    float p = on ? exp2f(x - mnew) : 0.f;
+    l = l * corr + p;
+#pragma unroll
+    for (int j = 0; j < kDims; ++j) o[j] *= corr;
+    m = mnew;
+    p = on ? p * a.c.v_scale[ph * kKv8Subs + slot / kKv8Block] : 0.f;
+    const uint8_t* vp = static_cast<const uint8_t*>(a.c.v) + (ph * kKv8Page + g * 32 % kKv8Page) * hd;
+    for (int kk = 0; kk < 32; ++kk) {
+      const float pk = __shfl_sync(0xffffffffu, p, kk);
+      if (g * 32 + kk < k0 || g * 32 + kk >= k1) continue;  // rows there may hold anything
+#pragma unroll
+      for (int j = 0; j < kDims; ++j)
+        if (lane + 32 * j < hd) o[j] += pk * e4m3_value(vp[(size_t)kk * hd + lane + 32 * j]);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (lane == 0) {
+    mw[warp] = m;
+    lw[warp] = l;
+  }
+#pragma unroll
+  for (int j = 0; j < kDims; ++j)
+    if (lane + 32 * j < hd) ow[warp][lane + 32 * j] = o[j];
+  __syncthreads();
+  float M = -INFINITY;
+  for (int w = 0; w < kGenWarps; ++w) M = fmaxf(M, mw[w]);
+  for (int d = threadIdx.x; d < hd; d += blockDim.x) {
+    float num = 0.f, den = 0.f;
+    for (int w = 0; w < kGenWarps; ++w) {
+      // a warp without a key has l = 0; one whose scores are all NaN has l = NaN
+      const float f = mw[w] == -INFINITY ? 1.f : exp2f(mw[w] - M);
+      num += f * ow[w][d];
+      den += f * lw[w];
+    }
+    out[d] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+  }
+}
+
+}  // namespace
+
+cudaError_t kv8_append(const Kv8AppendArgs& a, cudaStream_t s) {
+  // blocks that seq tokens can touch, wherever they begin
+  const int blocks = (a.seq + kKv8Block - 2) / kKv8Block + 1;
+  return launch_pdl(kv8_append_kernel, dim3(blocks, 2 * a.c.kv_heads, a.batch), dim3(128), 0, s, a);
+}
+
+cudaError_t kv8_attention(const Kv8AttnArgs& a, cudaStream_t s) {
+  const dim3 grid((unsigned)a.seq * a.heads, 1, a.batch);
+  return a.alibi ? launch_pdl(kv8_attn_rows_kernel<true>, grid, dim3(kGenWarps * 32), 0, s, a)
+                 : launch_pdl(kv8_attn_rows_kernel<false>, grid, dim3(kGenWarps * 32), 0, s, a);
+}
+
+}  // namespace wv

@@ -162,7 +162,8 @@ const char* err_reason(uint32_t code) {
   case kErrWaitAccEmpty: return "device wait timeout (accumulator empty)";
   case kErrWaitOther: return "device wait timeout";
   case kErrPeerWait: return "peer rank's data did not arrive (peer-memory all-reduce)";
-  case 0x100: return "RoPE position outside the table";
+  case kErrRopePos: return "RoPE position outside the table";
+  case kErrKvPage: return "KV block table names a page outside the pool or ends before the context";
   default: return "device error";
   }
 }

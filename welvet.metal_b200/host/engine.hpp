@@ -242,6 +242,11 @@ Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on
 Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* post,
                   bool on_device, cudaStream_t s);
 
+// Attention over an E4M3 cache (kv8.cpp): whether the configuration is built (code 2
+// otherwise), and its mask, scale and head shard as kernel arguments.
+Status kv8_supported(const Cfg& c, const char* who);
+void kv8_mask(const Cfg& c, Kv8AttnArgs* a);
+
 // NCCL (comm.cpp)
 Status comm_unique_id(uint8_t id[128]);
 Status comm_attach(Mha* m, const uint8_t id[128], int nranks, int rank);

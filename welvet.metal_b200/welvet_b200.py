@@ -44,7 +44,9 @@ EXT_SYMBOLS = ("welvet_b200_mha_config_default", "welvet_b200_mha_mount", "welve
                "welvet_b200_decode_attention_static", "welvet_b200_swiglu_mount", "welvet_b200_swiglu_forward",
                "welvet_b200_swiglu_forward_host", "welvet_b200_swiglu_release", "welvet_b200_norm_forward",
                "welvet_b200_embedding_forward", "welvet_b200_wait_probe", "welvet_b200_mha_set_output_mode",
-               "welvet_b200_attention_tf32")
+               "welvet_b200_attention_tf32", "welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward",
+               "welvet_b200_qk_norm_rope_workspace", "welvet_b200_qk_norm_rope_backward", "welvet_b200_kv8_append",
+               "welvet_b200_kv8_attention")
 PROFILE_SLOTS = ("gemm_qkv", "attn_prefill", "gemm_o", "attn_decode", "gemm_qkv_decode", "gemm_o_decode",
                  "allreduce", "other", "gemm_gate_up", "gemm_down", "norm", "embedding", "attn_bwd", "gemm_grad")
 
@@ -85,6 +87,12 @@ class MhaConfig(C.Structure):
         hd = self.head_dim if self.head_dim > 0 else self.d_model // self.num_heads
         nk = self.num_kv_heads if self.num_kv_heads > 0 else self.num_heads
         return hd, nk
+
+
+class _Kv8CacheArgs(C.Structure):
+    """welvet_b200_kv8_cache (include/welvet_b200.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "block_table", "ctx_len")] + [
+        (n, C.c_int32) for n in ("batch", "pages", "max_pages", "kv_heads", "head_dim")]
 
 
 _LIB = None
@@ -166,7 +174,18 @@ def lib():
     L.welvet_b200_wait_probe.argtypes = [C.c_uint64, _vp]
     L.welvet_b200_mha_set_output_mode.argtypes = [_vp, C.c_int32]
     L.welvet_b200_attention_tf32.argtypes = [cfgp, C.c_int32, C.c_int32] + [_vp] * 9 + [_vp]
-    for name in ("welvet_b200_wait_probe", "welvet_b200_mha_set_output_mode", "welvet_b200_attention_tf32",
+    kv8p = C.POINTER(_Kv8CacheArgs)
+    L.welvet_b200_rope_table.argtypes = [C.c_int32, C.c_int32, C.c_double, _vp, _vp]
+    norm = [C.c_int64] + [C.c_int32] * 3 + [C.c_double, _vp, _vp, _vp, C.c_int32, _vp, C.c_int32] + [_vp, C.c_int64] * 4
+    L.welvet_b200_qk_norm_rope_forward.argtypes = norm + [C.c_int32, _vp]
+    L.welvet_b200_qk_norm_rope_workspace.argtypes = [C.c_int32]
+    L.welvet_b200_qk_norm_rope_workspace.restype = C.c_int64
+    L.welvet_b200_qk_norm_rope_backward.argtypes = norm + [_vp, C.c_int64] * 2 + [_vp] * 3 + [C.c_int32, _vp]
+    L.welvet_b200_kv8_append.argtypes = [kv8p, C.c_int32, _vp, _vp, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, _vp]
+    L.welvet_b200_kv8_attention.argtypes = [cfgp, kv8p, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, _vp]
+    for name in ("welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward", "welvet_b200_qk_norm_rope_backward",
+                 "welvet_b200_kv8_append", "welvet_b200_kv8_attention",
+                 "welvet_b200_wait_probe", "welvet_b200_mha_set_output_mode", "welvet_b200_attention_tf32",
 "welvet_b200_mha_mount", "welvet_b200_mha_forward", "welvet_b200_mha_forward_rows",
                  "welvet_b200_mha_check",
                  "welvet_b200_kv_create", "welvet_b200_kv_fill", "welvet_b200_mha_prefill",
@@ -203,6 +222,16 @@ def _ptr(a):
     if isinstance(a, int):
         return a
     raise TypeError(type(a))
+
+
+def _rows(t, width):
+    """(pointer, row stride) of a 2-D device tensor of at least `width` values a row, the
+    values of a row next to each other; (None, width) for None."""
+    if t is None:
+        return None, width
+    if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] < width:
+        raise ValueError(f"rows of at least {width} adjacent values expected, got {tuple(t.shape)}")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]))
 
 
 def _stream(s):
@@ -492,6 +521,114 @@ def attention_tf32(cfg: MhaConfig, batch, seq, q, q_lo, k, k_lo, v, v_lo, out, o
     check(lib().welvet_b200_attention_tf32(C.byref(cfg), batch, seq, _ptr(q), _ptr(q_lo), _ptr(k), _ptr(k_lo),
                                            _ptr(v), _ptr(v_lo), _ptr(out), _ptr(out_hi), _ptr(out_lo),
                                            _stream(stream)))
+
+
+def rope_table(max_pos, head_dim, table, theta=10000.0, stream=None):
+    """(cos, sin) of pos / theta^(2i/head_dim) into table [max_pos, head_dim/2, 2] FP32."""
+    check(lib().welvet_b200_rope_table(max_pos, head_dim, theta, _typed(table, "torch.float32", max_pos * head_dim),
+                                       _stream(stream)))
+
+
+def _typed(t, dtype, numel=0):
+    """Device pointer of a contiguous tensor of the given dtype and at least numel values."""
+    if t is None:
+        return None
+    if str(t.dtype) != dtype or not t.is_contiguous() or t.numel() < numel:
+        raise ValueError(f"contiguous {dtype} of at least {numel} values expected, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _norm_call(q, k, q_out, k_out, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod):
+    tokens = q.shape[0]
+    for t in (k, q_out, k_out):
+        if t is not None and (t.shape[0] != tokens or t.dtype != q.dtype):
+            raise ValueError("q, k and their outputs need the same tokens and dtype")
+    io = {"torch.bfloat16": 1, "torch.float32": 0}.get(str(q.dtype))
+    if io is None or q.shape[1] % head_dim or (k is not None and k.shape[1] % head_dim):
+        raise ValueError("BF16 or FP32 rows of whole heads expected")
+    heads, kv_heads = q.shape[1] // head_dim, 0 if k is None else k.shape[1] // head_dim
+    args = [tokens, heads, kv_heads, head_dim, eps, _typed(q_gamma, "torch.float32", head_dim),
+            _typed(k_gamma, "torch.float32", head_dim), _typed(rope, "torch.float32"),
+            0 if rope is None else rope.numel() // head_dim, _typed(positions, "torch.int32", tokens), pos_mod,
+            *_rows(q, heads * head_dim), *_rows(k, kv_heads * head_dim)]
+    return io, args, (heads * head_dim, kv_heads * head_dim)
+
+
+def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1e-6, rope=None, positions=None,
+                 pos_mod=0, stream=None):
+    """RMS norm of every query and key head with the rotation in the same pass
+    (welvet_b200_qk_norm_rope_forward): rows [tokens, heads * head_dim] (may be views of
+    one packed row; k may be None), outputs may be the inputs."""
+    io, args, (qd, kd) = _norm_call(q, k, q_out, k_out, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    check(lib().welvet_b200_qk_norm_rope_forward(*args, *_rows(q_out, qd), *_rows(k_out, kd), io, _stream(stream)))
+
+
+def qk_norm_rope_workspace(head_dim) -> int:
+    """Bytes of the workspace of qk_norm_rope_backward."""
+    return int(lib().welvet_b200_qk_norm_rope_workspace(head_dim))
+
+
+def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, dq_gamma, dk_gamma, head_dim, workspace, q_gamma=None,
+                          k_gamma=None, eps=1e-6, rope=None, positions=None, pos_mod=0, stream=None):
+    """Gradient of qk_norm_rope (welvet_b200_qk_norm_rope_backward): dq, dk from the
+    forward's inputs and the gradients of its outputs, dq_gamma / dk_gamma [head_dim]
+    overwritten with the sums over all rows."""
+    io, args, (qd, kd) = _norm_call(q, k, dq, dk, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    for t in (dq_out, dk_out):
+        if t is not None and (t.shape[0] != q.shape[0] or t.dtype != q.dtype):
+            raise ValueError("the gradients need the tokens and dtype of q")
+    if workspace.numel() * workspace.element_size() < qk_norm_rope_workspace(head_dim):
+        raise ValueError("workspace smaller than qk_norm_rope_workspace(head_dim)")
+    check(lib().welvet_b200_qk_norm_rope_backward(
+        *args, *_rows(dq_out, qd), *_rows(dk_out, kd), *_rows(dq, qd), *_rows(dk, kd),
+        _typed(dq_gamma, "torch.float32", head_dim), _typed(dk_gamma, "torch.float32", head_dim), _ptr(workspace), io,
+        _stream(stream)))
+
+
+class Kv8Cache:
+    """The caller's tensors of a paged E4M3 cache (welvet_b200_kv8_cache): codes k, v
+    [pages, kv_heads, 64, head_dim] (one byte each), scales [pages, kv_heads, 4] FP32,
+    block_table [batch, max_pages] and ctx_len [batch] int32, the lengths with the new
+    tokens included."""
+    PAGE, BLOCK = 64, 16
+
+    def __init__(self, k, v, k_scale, v_scale, block_table, ctx_len):
+        pages, kv_heads, page, head_dim = k.shape
+        if page != self.PAGE or v.shape != k.shape or k.element_size() != 1 or v.element_size() != 1:
+            raise ValueError("codes [pages, kv_heads, 64, head_dim] of one byte expected")
+        batch, max_pages = block_table.shape
+        n = pages * kv_heads * (self.PAGE // self.BLOCK)
+        self.tensors = (k, v, k_scale, v_scale, block_table, ctx_len)
+        self.args = _Kv8CacheArgs(_ptr(k), _ptr(v), _typed(k_scale, "torch.float32", n),
+                                  _typed(v_scale, "torch.float32", n), _typed(block_table, "torch.int32"),
+                                  _typed(ctx_len, "torch.int32", batch), batch, pages, max_pages, kv_heads, head_dim)
+
+
+def _bf16_rows(t, rows, width):
+    if str(t.dtype) != "torch.bfloat16" or t.shape[0] < rows:
+        raise ValueError(f"{rows} BF16 rows expected, got {t.dtype} {tuple(t.shape)}")
+    return _rows(t, width)
+
+
+def kv8_append(cache: Kv8Cache, seq, k, v, rope=None, seq_lens=None, stream=None):
+    """Appends rows b * seq + t of k and v (BF16 [batch * seq, kv_heads * head_dim], may be
+    views of packed rows) to the cache (welvet_b200_kv8_append)."""
+    c = cache.args
+    width = c.kv_heads * c.head_dim
+    check(lib().welvet_b200_kv8_append(C.byref(c), seq, _typed(seq_lens, "torch.int32", c.batch),
+                                       *_bf16_rows(k, c.batch * seq, width), *_bf16_rows(v, c.batch * seq, width),
+                                       _typed(rope, "torch.float32"), 0 if rope is None else rope.numel() // c.head_dim,
+                                       _stream(stream)))
+
+
+def kv8_attention(cfg: MhaConfig, cache: Kv8Cache, seq, q, out, max_ctx, seq_lens=None, stream=None):
+    """Attention of the new tokens (BF16 rows b * seq + t of q) over the cache
+    (welvet_b200_kv8_attention)."""
+    c = cache.args
+    width = (cfg.head_count if cfg.head_count > 0 else cfg.num_heads) * c.head_dim
+    check(lib().welvet_b200_kv8_attention(C.byref(cfg), C.byref(c), seq, _typed(seq_lens, "torch.int32", c.batch),
+                                          max_ctx, *_bf16_rows(q, c.batch * seq, width),
+                                          *_bf16_rows(out, c.batch * seq, width), _stream(stream)))
 
 
 def codec_roundtrip(dtype, w, out, stream=None):
