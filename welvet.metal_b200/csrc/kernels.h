@@ -367,7 +367,11 @@ struct Kv8AttnArgs {
   uint32_t* err = nullptr;
   int sm_count = 148;
 };
+// The tensor-core kernel (kv8_attn.cu: head_dim 64 / 128, 16-byte aligned codes and
+// scales), or the general one (kv8.cu).
 cudaError_t kv8_attention(const Kv8AttnArgs& a, cudaStream_t s);
+bool kv8_attention_tc_supported(const Kv8AttnArgs& a);
+cudaError_t kv8_attention_tc(const Kv8AttnArgs& a, cudaStream_t s);
 
 // ---- transformer-block kernels (block.cu)
 struct NormArgs {

@@ -190,6 +190,7 @@ cudaError_t kv8_append(const Kv8AppendArgs& a, cudaStream_t s) {
 }
 
 cudaError_t kv8_attention(const Kv8AttnArgs& a, cudaStream_t s) {
+  if (kv8_attention_tc_supported(a)) return kv8_attention_tc(a, s);
   const dim3 grid((unsigned)a.seq * a.heads, 1, a.batch);
   return a.alibi ? launch_pdl(kv8_attn_rows_kernel<true>, grid, dim3(kGenWarps * 32), 0, s, a)
                  : launch_pdl(kv8_attn_rows_kernel<false>, grid, dim3(kGenWarps * 32), 0, s, a);

@@ -1,0 +1,637 @@
+// Attention over the paged E4M3 KV cache on the 5th-generation tensor cores: head_dim
+// 64 and 128, from one new token per sequence to prompt chunks.
+//
+// The codes are never widened. With the keys as the 128-row operand, both products run
+// as FP8 UMMAs on the tiles as TMA brings them from the pages:
+//   S^T [128 keys, columns] = K [128 keys, hd] (A, E4M3, K-major) * Q^T
+//   O^T [hd, columns]      += V^T (A, E4M3, MN-major: the same [key][hd] bytes) * P^T
+// A column is one (new token, query head of the KV group); RT of them share a CTA's
+// pass over the keys, so a decode step needs a 16-column MMA and no padding of queries
+// to 128 rows, and a thread of the softmax holds one key of every column: no work is
+// spent on absent queries, and no row reductions across lanes are needed per tile.
+// What the small operands lose in 8 bits is kept in more columns (columns are nearly
+// free while the 128-row operand sets the pace):
+//   * a query row, scaled by a power of two to at most 448, is hi + lo/16, two E4M3
+//     codes: exact to 2^-14 or better of 448, i.e. BF16 queries to 2^-22 of the row's
+//     largest value;
+//   * a probability is hi + lo/8 + lo2/64, three E5M2 codes (3 significant bits each,
+//     rounded to nearest in turn): a relative 2^-10, down to 2^-28 of the largest
+//     before the codes run out, so that long tails of small probabilities still add
+//     up. E4M3 codes would be finer but end at 2^-16 of the largest.
+// Scores and sums are FP32 (TMEM accumulators, registers).
+//
+// Softmax in the log2 domain with the value scale folded in: z = s kscale qscale
+// scale log2e + log2(vscale), p = 2^(z - ref), O += p * code, l += p / vscale. ref is a
+// column's running maximum of z, raised only when some z exceeds it by more than 2^8
+// (E5M2 has the room), so that most tiles need one vote and no maximum at all; when
+// it moves, the CTA's O and l are rescaled.
+//
+// Roles: one or two softmax warpgroups (a column group each; thread = TMEM lane =
+// key), a TMA warp (pages of codes and their four scales into a ring of 128-key
+// stages), an MMA warp (S_0, S_1, then PV_i, S_{i+2}; S and P double-buffered).
+// A long context is split over a cluster of up to 16 CTAs whose partial (ref, l, O)
+// are joined through distributed shared memory in rank order: no workspace, no second
+// launch, the same bits every time.
+// Masked keys and rows past the context: their p is set to 0 and their V rows cleared
+// (a byte never written may be a NaN code); NaN scales reach only columns that see them.
+#include "attn_common.cuh"
+#include "kv8.cuh"
+
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <climits>
+
+namespace wv {
+namespace {
+
+constexpr int kKeys = 128;          // keys of a tile: two pages
+constexpr float kBias = 6.f;        // log2 of p at the reference
+constexpr float kSlack = 8.f;       // z may exceed the reference by this much
+constexpr float kNoRef = 1e30f;     // bias - ref of a column that has seen no key
+constexpr int kMaxCluster = 16;
+
+template <int HD, int RT> struct KT {
+  static constexpr int NWG = RT > 16 ? 2 : 1;       // softmax warpgroups
+  static constexpr int CPW = RT / NWG;              // columns of one
+  static constexpr int THREADS = NWG * 128 + 64;
+  static constexpr int TILE = kKeys * HD;           // bytes of a K or V tile
+  static constexpr int STAGE = 2 * TILE;
+  // 512 TMEM columns (RT = 64) take the SM for one CTA; the deeper ring then takes its
+  // shared memory too, so that no other CTA of these kernels waits there for columns.
+  static constexpr int STAGES = (HD == 64 ? 4 : 3) + (RT == 64 ? (HD == 64 ? 4 : 1) : 0);
+  static constexpr int NS = 2 * RT;                 // columns of S: hi | lo
+  static constexpr int NP = RT == 8 ? 32 : 3 * RT;  // columns of P and O: hi | lo | lo2
+  static constexpr int P_BYTES = kKeys * NP;
+  static constexpr int Q_BYTES = NS * HD;
+  static constexpr int TMEM = RT == 8 ? 64 : RT == 16 ? 128 : RT == 32 ? 256 : 512;
+  static constexpr int O_COL = 2 * NS;              // TMEM: S_0 | S_1 | O
+  static constexpr int OFF_P = STAGES * STAGE;
+  static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
+  static constexpr int OFF_SC = OFF_Q + Q_BYTES;    // scales: [stage][K, V][8]
+  static constexpr int OFF_COL = OFF_SC + STAGES * 64;  // per column: (factor, bias - ref)
+  static constexpr int OFF_QHI = OFF_COL + RT * 8;      // last key of a column
+  static constexpr int OFF_SLOPE = OFF_QHI + RT * 4;
+  static constexpr int OFF_L = OFF_SLOPE + RT * 4;      // sums of the CTA
+  static constexpr int OFF_RED = OFF_L + RT * 4;        // [4 warps][RT]
+  static constexpr int OFF_BAR = OFF_RED + 4 * RT * 4;
+  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (2 * STAGES + 6) + 32;
+  // resident CTAs of an SM
+  static constexpr int BY_SMEM = 228 * 1024 / (SMEM + 1024), BY_TMEM = 512 / TMEM;
+  static constexpr int PER_SM = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
+  // Partial O of a split, [RT][HD] FP32, over the stages once every MMA has read them.
+  static_assert(RT * HD * 4 <= STAGES * STAGE, "partial outputs over the stages");
+  static_assert(O_COL + NP <= TMEM, "TMEM columns");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+// D[tmem] (+)= A[smem] B[smem]^T with 8-bit operands; descriptors as 32-bit halves.
+WV_DEV void umma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                    uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// High descriptor word: stride byte offset, version 1, layout type (0 none, 2 128-byte,
+// 4 64-byte swizzle).
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo_bytes, uint32_t layout) {
+  return ((sbo_bytes >> 4) & 0x3FFFu) | (1u << 14) | (layout << 29);
+}
+// Instruction descriptor of kind::f8f6f4, FP32 accumulators; formats: 0 E4M3, 1 E5M2.
+__host__ __device__ constexpr uint32_t idesc_f8(uint32_t a_fmt, uint32_t b_fmt, int M, int N, uint32_t a_mn, uint32_t b_mn) {
+  return (1u << 4) | (a_fmt << 7) | (b_fmt << 10) | (a_mn << 15) | (b_mn << 16) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
+
+// N consecutive TMEM columns of this thread's lane.
+template <int N> WV_DEV void tmem_ld(uint32_t addr, uint32_t* r) {
+  if constexpr (N == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+  } else if constexpr (N == 16) {
+    tmem_ld16(addr, *reinterpret_cast<uint32_t(*)[16]>(r));
+  } else {
+    tmem_ld32(addr, *reinterpret_cast<uint32_t(*)[32]>(r));
+  }
+}
+template <int N> WV_DEV void tmem_st(uint32_t addr, const uint32_t* r) {
+  if constexpr (N == 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else if constexpr (N == 16) {
+    tmem_st16(addr, *reinterpret_cast<const uint32_t(*)[16]>(r));
+  } else {
+    tmem_st32(addr, *reinterpret_cast<const uint32_t(*)[32]>(r));
+  }
+}
+// Maximum over the warp; NaN lanes are left out.
+WV_DEV float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Barrier of a warpgroup that also says whether any thread's predicate holds.
+template <int ID> WV_DEV bool bar_any(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "n"(ID)
+      : "memory");
+  return r != 0;
+}
+template <int ID> WV_DEV void bar_sync() { asm volatile("barrier.cta.sync %0, 128;" ::"n"(ID) : "memory"); }
+template <int NWG> WV_DEV bool wg_any(int wg, bool v) { return NWG == 1 || wg == 0 ? bar_any<1>(v) : bar_any<2>(v); }
+template <int NWG> WV_DEV void wg_sync(int wg) {
+  if (NWG == 1 || wg == 0) bar_sync<1>();
+  else bar_sync<2>();
+}
+// Two FP32 values as E5M2 codes (nearest, saturating), and the values of two codes: an
+// E5M2 code is the upper byte of the FP16 pattern of its value.
+WV_DEV uint32_t e5m2x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+WV_DEV float2 e5m2x2_value(uint32_t c) {
+  const uint32_t h = __byte_perm(c, 0u, 0x1404);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+WV_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+WV_DEV uint32_t peer_addr(const void* local, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+  return r;
+}
+WV_DEV float ld_peer(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int HD, int RT, bool ALIBI>
+__global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
+    kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const Kv8AttnArgs a, int splits) {
+  using T = KT<HD, RT>;
+  constexpr int CPW = T::CPW, ST = T::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::OFF_BAR);
+  uint64_t* empty = full + ST;
+  uint64_t* s_full = empty + ST;  // [2]
+  uint64_t* p_full = s_full + 2;  // [2]
+  uint64_t* pv_done = p_full + 2; // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float2* col = reinterpret_cast<float2*>(smem + T::OFF_COL);
+  int* qhi = reinterpret_cast<int*>(smem + T::OFF_QHI);
+  float* slope = reinterpret_cast<float*>(smem + T::OFF_SLOPE);
+  float* lsum = reinterpret_cast<float*>(smem + T::OFF_L);
+  float* red = reinterpret_cast<float*>(smem + T::OFF_RED);
+  const int warp = (int)warp_id(), lane = (int)lane_id();
+  constexpr int kSoftWarps = T::NWG * 4;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kSoftWarps);
+      mbar_init(&pv_done[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kSoftWarps) {
+    tmem_alloc(tmem_holder, T::TMEM);
+    tmem_relinquish();
+  }
+  pdl_wait();  // the append (or whatever filled the cache, q and the lengths) is complete
+
+  // ---- this CTA's columns and keys
+  const int split = blockIdx.x % splits, b = blockIdx.z;
+  const int kh = blockIdx.y, r0 = (int)(blockIdx.x / splits) * RT;
+  const int G = a.heads / a.c.kv_heads;
+  const int n = kv8_new(a.seq_lens, b, a.seq);
+  int ctx = a.c.ctx_len[b];
+  const int shift = ctx - n;  // position of the first new token
+  const int t0 = max(r0 / G, max(0, -shift)), t1 = min((r0 + RT - 1) / G, n - 1);  // live tokens
+  const int qlo = shift + t0;
+  int k1 = t1 >= t0 ? shift + t1 + 1 : 0;
+  if (k1 > a.c.max_pages * kKv8Page) {
+    if (threadIdx.x == 0) atomicCAS(a.err, 0u, kErrKvPage);
+    k1 = a.c.max_pages * kKv8Page;
+  }
+  const int page0 = (a.window > 0 ? max(0, qlo + 1 - a.window) : 0) / kKv8Page;
+  const int all = k1 > page0 * kKv8Page ? (k1 - page0 * kKv8Page + kKeys - 1) / kKeys : 0;
+  const int per = (all + splits - 1) / splits;
+  const int tile0 = min(all, split * per), tiles = min(all, tile0 + per) - tile0;
+  const int base0 = page0 * kKv8Page + tile0 * kKeys;  // first key of tile 0
+
+  // ---- queries: hi and lo codes, [16-byte chunk of hd][2 RT rows][16]
+  if (warp < kSoftWarps) {
+    for (int c = warp; c < RT; c += kSoftWarps) {
+      const int t = (r0 + c) / G, h = kh * G + (r0 + c) % G;
+      const bool live = t >= t0 && t <= t1;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + t) * a.ldq + (size_t)h * HD;
+      float x[HD / 32], m = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        x[i] = live ? __bfloat162float(q[lane + 32 * i]) : 0.f;
+        m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
+      }
+      m = warp_max(m);
+      const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
+      const float s = bad ? 1.f : kv8_scale(m);
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const int e = lane + 32 * i;
+        const float y = bad ? 0.f : x[i] / s;
+        const uint32_t hi = e4m3x2(y, 0.f);
+        const uint32_t lo = e4m3x2((y - e4m3x2_value(hi).x) * 16.f, 0.f);
+        uint8_t* dst = smem + T::OFF_Q + (e / 16) * (T::NS * 16) + e % 16;
+        dst[c * 16] = (uint8_t)hi;
+        dst[(RT + c) * 16] = (uint8_t)lo;
+      }
+      if (lane == 0) {
+        col[c] = make_float2(bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e, kNoRef);
+        qhi[c] = live ? min(shift + t, k1 - 1) : k1 - 1;  // a column without a query sees whatever there is
+        if (ALIBI) slope[c] = exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * kLog2e;
+      }
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  pdl_trigger();  // behind the TMEM allocation: a dependent's CTA must not take the columns first
+  bool ok = true;
+  float l[CPW];
+#pragma unroll
+  for (int c = 0; c < CPW; ++c) l[c] = 0.f;
+
+  if (warp == kSoftWarps) {
+    // ------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    const int* bt = a.c.block_table + (size_t)b * a.c.max_pages;
+    const int p0 = base0 / kKv8Page;
+    const int np = tiles > 0 ? min((k1 + kKv8Page - 1) / kKv8Page - p0, 2 * tiles) : 0;  // pages of this CTA
+    int next = lane < np ? bt[p0 + lane] : 0, ids = 0;
+    for (int j = 0; j < tiles; ++j) {
+      if (j % 16 == 0) {  // 32 page ids at a time, requested one batch ahead
+        ids = next;
+        const int at = 2 * j + 32 + lane;
+        next = at < np ? bt[p0 + at] : 0;
+        if (ids < 0 || ids >= a.c.pages) {  // reported; page 0 in its place keeps every access inside
+          if (2 * j + lane < np) atomicCAS(a.err, 0u, kErrKvPage);
+          ids = 0;
+        }
+      }
+      const int s = j % ST;
+      if (ok && lane == 0 && j >= ST) ok = mbar_wait(&empty[s], ((j / ST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (!ok) {  // the copies in flight land before the CTA ends (bounded)
+        int none = 0;
+        for (int k = max(0, j - ST); lane == 0 && k < j; ++k)
+          mbar_wait_for(&full[k % ST], (k / ST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
+        break;
+      }
+      const int two = 2 * j + 1 < np ? 2 : 1;
+      const int id[2] = {__shfl_sync(0xffffffffu, ids, (2 * j) & 31), __shfl_sync(0xffffffffu, ids, (2 * j + 1) & 31)};
+      if (lane == 0) {
+        uint8_t* kt = smem + s * T::STAGE;
+        float* sc = reinterpret_cast<float*>(smem + T::OFF_SC + s * 64);
+        mbar_arrive_expect_tx(&full[s], two * (2 * kKv8Page * HD + 32));
+        for (int i = 0; i < two; ++i) {
+          const int ph = id[i] * a.c.kv_heads + kh;
+          tma_load_2d(kt + i * kKv8Page * HD, &tmK, &full[s], 0, ph * kKv8Page);
+          bulk_load(sc + i * 4, a.c.k_scale + (size_t)ph * kKv8Subs, 16, &full[s]);
+          tma_load_2d(kt + T::TILE + i * kKv8Page * HD, &tmV, &full[s], 0, ph * kKv8Page);
+          bulk_load(sc + 8 + i * 4, a.c.v_scale + (size_t)ph * kKv8Subs, 16, &full[s]);
+        }
+      }
+    }
+  } else if (warp == kSoftWarps + 1) {
+    // --------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kRow = HD == 128 ? 2u : 4u;  // swizzle of the code tiles
+      constexpr uint32_t HI_KV = desc_hi(8 * HD, kRow);       // 8 keys of HD bytes
+      constexpr uint32_t HI_Q = desc_hi(128, 0);              // 8 rows of 16 bytes
+      constexpr uint32_t HI_P = desc_hi(kKeys * 16, 0);       // 16 columns of every key
+      constexpr uint32_t IDESC_S = idesc_f8(0, 0, 128, T::NS, 0, 0);
+      constexpr uint32_t IDESC_PV = idesc_f8(0, 1, HD, T::NP, 1, 1);
+      const uint32_t q_lo = sdesc_lo(smem_u32(smem + T::OFF_Q), T::NS * 16);
+      auto issue_s = [&](int j) -> bool {
+        const int s = j % ST;
+        if (!mbar_wait(&full[s], (j / ST) & 1, abort_flag, a.err, kErrWaitFull)) return false;
+        tc_fence_after();
+        const uint32_t k_lo = sdesc_lo(smem_u32(smem + s * T::STAGE), 16);
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk)
+          umma_f8(tmem + (uint32_t)((j & 1) * T::NS), k_lo + kk * 2, HI_KV, q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
+        umma_commit(&s_full[j & 1]);
+        return true;
+      };
+      for (int j = 0; ok && j < min(2, tiles); ++j) ok = issue_s(j);
+      for (int i = 0; ok && i < tiles; ++i) {
+        ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitOther);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v_lo = sdesc_lo(smem_u32(smem + (i % ST) * T::STAGE + T::TILE), 16);
+        const uint32_t p_lo = sdesc_lo(smem_u32(smem + T::OFF_P + (i & 1) * T::P_BYTES), 128);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 32; ++kk)
+          umma_f8(tmem + T::O_COL, v_lo + kk * (32 * HD / 16), HI_KV, p_lo + kk * (32 * 16 / 16), HI_P, IDESC_PV,
+                  (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&empty[i % ST]);
+        umma_commit(&pv_done[i & 1]);
+        if (i + 2 < tiles) ok = issue_s(i + 2);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int wg = warp >> 2, w4 = warp & 3;
+    const int key = 32 * w4 + lane;  // of the tile; this thread's TMEM lane
+    const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16);
+    const int c0 = wg * CPW;
+    for (int i = 0; i < tiles; ++i) {
+      const int s = i % ST, base = base0 + i * kKeys, kpos = base + key;
+      // After a wait that gave up, the tiles are still walked (the waits return at once):
+      // the warpgroup's barriers need every thread.
+      ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
+      ok = mbar_wait(&full[s], (i / ST) & 1, abort_flag, a.err, kErrWaitFull) && ok;  // its scales
+      tc_fence_after();
+      const float* sc = reinterpret_cast<const float*>(smem + T::OFF_SC + s * 64);
+      const bool on = kpos < k1;
+      const float ks = sc[key >> 4], vs = sc[8 + (key >> 4)];
+      float ev, inv;
+      asm("lg2.approx.f32 %0, %1;" : "=f"(ev) : "f"(vs));
+      inv = on && vs == vs ? __frcp_rn(vs) : 0.f;
+      if (!on && wg == 0) {  // rows past the context may hold NaN codes: 0 * NaN
+        uint8_t* row = smem + s * T::STAGE + T::TILE + key * HD;
+#pragma unroll
+        for (int x = 0; x < HD; x += 16) *reinterpret_cast<uint4*>(row + x) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      // z of this key for the group's columns
+      float z[CPW];
+      {
+        uint32_t hi[CPW], lo[CPW];
+        tmem_ld<CPW>(tl + (i & 1) * T::NS + c0, hi);
+        tmem_ld<CPW>(tl + (i & 1) * T::NS + RT + c0, lo);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < CPW; ++c)
+          z[c] = fmaf(fmaf(__uint_as_float(lo[c]), 0.0625f, __uint_as_float(hi[c])) * ks, col[c0 + c].x, ev);
+      }
+      if (ALIBI) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) z[c] -= slope[c0 + c] * (float)(qhi[c0 + c] - kpos);
+      }
+      if (base + kKeys > qlo + 1 || (a.window > 0 && base <= k1 - 1 - a.window)) {  // some column's edge
+#pragma unroll
+        for (int c = 0; c < CPW; ++c)
+          if (kpos > qhi[c0 + c] || (a.window > 0 && kpos <= qhi[c0 + c] - a.window)) z[c] = -INFINITY;
+      }
+      bool high = false;
+#pragma unroll
+      for (int c = 0; c < CPW; ++c) high |= z[c] + col[c0 + c].y > kBias + kSlack;
+      if (i >= 2) ok = mbar_wait(&pv_done[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;  // P is free
+      if (wg_any<T::NWG>(wg, high)) {
+        // new references: the maximum of every column over the tile's keys
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) {
+          const float m = warp_max(z[c]);
+          if (lane == 0) red[w4 * RT + c0 + c] = m;
+        }
+        // O holds PV_{i-1}
+        if (i > 0) ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+        tc_fence_after();
+        wg_sync<T::NWG>(wg);
+        float f[CPW], ref[CPW];
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) {
+          const int cc = c0 + c;
+          const float m = fmaxf(fmaxf(red[cc], red[RT + cc]), fmaxf(red[2 * RT + cc], red[3 * RT + cc]));
+          const float was = col[cc].y, now = m == -INFINITY ? was : fminf(was, kBias - m);
+          f[c] = was == kNoRef ? 1.f : fast_exp2(now - was);
+          ref[c] = now;
+          l[c] *= f[c];
+        }
+        wg_sync<T::NWG>(wg);  // every thread has read the old references
+#pragma unroll
+        for (int c = 0; c < CPW; ++c)
+          if (key == c) col[c0 + c].y = ref[c];
+        if (i > 0) {
+#pragma unroll
+          for (int term = 0; term < 3; ++term) {
+            uint32_t o[CPW];
+            tmem_ld<CPW>(tl + T::O_COL + term * RT + c0, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < CPW; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f[c]);
+            tmem_st<CPW>(tl + T::O_COL + term * RT + c0, o);
+          }
+          tmem_st_wait();
+        }
+        wg_sync<T::NWG>(wg);  // the new references are in place
+      }
+      // probabilities, and their three codes: chunks of 16 columns (of 8 + 8 when RT = 8)
+      uint32_t code[3][CPW / 4];
+#pragma unroll
+      for (int c = 0; c < CPW; c += 4) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = fast_exp2(z[c + e] + col[c0 + c + e].y);
+          l[c + e] = fmaf(p[e], inv, l[c + e]);
+        }
+#pragma unroll
+        for (int term = 0; term < 3; ++term) {
+          const uint32_t u = e5m2x2(p[0], p[1]), w = e5m2x2(p[2], p[3]);
+          code[term][c / 4] = u | (w << 16);
+          if (term < 2) {
+            const float2 x = e5m2x2_value(u), y = e5m2x2_value(w);
+            p[0] = (p[0] - x.x) * 8.f;
+            p[1] = (p[1] - x.y) * 8.f;
+            p[2] = (p[2] - y.x) * 8.f;
+            p[3] = (p[3] - y.y) * 8.f;
+          }
+        }
+      }
+      uint8_t* pt = smem + T::OFF_P + (i & 1) * T::P_BYTES + key * 16;
+      if constexpr (RT == 8) {
+        st_shared_v4(pt, code[0][0], code[0][1], code[1][0], code[1][1]);
+        st_shared_v4(pt + kKeys * 16, code[2][0], code[2][1], 0u, 0u);
+      } else {
+#pragma unroll
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+          for (int x = 0; x < CPW / 16; ++x)
+            st_shared_v4(pt + ((term * RT + c0) / 16 + x) * (kKeys * 16), code[term][4 * x], code[term][4 * x + 1],
+                         code[term][4 * x + 2], code[term][4 * x + 3]);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[i & 1]);
+    }
+    if (tiles > 0)
+      ok = mbar_wait(&pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+    tc_fence_after();
+    // sums of the columns over the keys of the four warps, in warp order
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) {
+      float v = l[c];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) red[w4 * RT + c0 + c] = v;
+    }
+    wg_sync<T::NWG>(wg);
+    if (key < CPW) lsum[c0 + key] = (red[c0 + key] + red[RT + c0 + key]) + (red[2 * RT + c0 + key] + red[3 * RT + c0 + key]);
+  }
+  // A bounded wait that gave up is in the error word: every thread still takes the
+  // barriers below, and the outputs are not written.
+  ok = __syncthreads_and(ok ? 1 : 0) != 0;
+
+  if (warp < kSoftWarps) {
+    // O^T: lane = dim (head_dim 64: 16 lanes of every warp), a column group per warpgroup
+    const int wg = warp >> 2, w4 = warp & 3, c0 = wg * CPW;
+    const int dim = HD == 128 ? 32 * w4 + lane : 16 * w4 + lane;
+    const bool mine = HD == 128 || lane < 16;
+    const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + T::O_COL + c0;
+    float o[CPW];
+    {
+      uint32_t x[CPW], y[CPW], w[CPW];
+      tmem_ld<CPW>(tl, x);
+      tmem_ld<CPW>(tl + RT, y);
+      tmem_ld<CPW>(tl + 2 * RT, w);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < CPW; ++c)
+        o[c] = tiles > 0 ? fmaf(fmaf(__uint_as_float(w[c]), 0.125f, __uint_as_float(y[c])), 0.125f, __uint_as_float(x[c])) : 0.f;
+    }
+    if (splits == 1) {
+      if (ok && mine) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) {
+          const int r = r0 + c0 + c, t = r / G;
+          if (t >= a.seq) break;
+          const float den = lsum[c0 + c];
+          const bool live = t >= t0 && t <= t1;
+          static_cast<__nv_bfloat16*>(a.out)[((size_t)b * a.seq + t) * a.ldo + (size_t)(kh * G + r % G) * HD + dim] =
+              __float2bfloat16_rn(!live || den == 0.f ? 0.f : o[c] / den);
+        }
+      }
+    } else if (mine) {
+      float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int c = 0; c < CPW; ++c) part[(c0 + c) * HD + dim] = o[c];
+    }
+  }
+  if (splits > 1) {
+    cluster_sync();
+    // joined in rank order: 2^(ref_s - ref) of every split's O and l, (column, dim)
+    // pairs dealt out over the cluster
+    for (int idx = split * T::THREADS + threadIdx.x; idx < RT * HD; idx += splits * T::THREADS) {
+      const int c = idx / HD, r = r0 + c, t = r / G;
+      if (t >= a.seq) break;
+      float ref = kNoRef, num = 0.f, den = 0.f;
+      for (int s = 0; s < splits; ++s) ref = fminf(ref, ld_peer(peer_addr(&col[c].y, s)));
+      for (int s = 0; s < splits; ++s) {
+        const float f = fast_exp2(ref - ld_peer(peer_addr(&col[c].y, s)));
+        num = fmaf(f, ld_peer(peer_addr(reinterpret_cast<float*>(smem) + idx, s)), num);
+        den = fmaf(f, ld_peer(peer_addr(&lsum[c], s)), den);
+      }
+      const bool live = t >= t0 && t <= t1;
+      if (ok)
+        static_cast<__nv_bfloat16*>(a.out)[((size_t)b * a.seq + t) * a.ldo + (size_t)(kh * G + r % G) * HD + idx % HD] =
+            __float2bfloat16_rn(!live || den == 0.f ? 0.f : num / den);
+    }
+    cluster_sync();  // no CTA leaves while another reads its partials
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps) tmem_dealloc(tmem, T::TMEM);
+}
+
+template <int HD, int RT> cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
+  using T = KT<HD, RT>;
+  const int group = a.heads / a.c.kv_heads;
+  const int64_t row_tiles = ((int64_t)a.seq * group + RT - 1) / RT;
+  const int64_t pairs = row_tiles * a.c.kv_heads * a.batch;
+  // One wave of resident CTAs: a context is split while the grid leaves SMs idle, down
+  // to one 128-key tile a CTA.
+  const int keys = a.window > 0 ? std::min(a.max_ctx, a.window + a.seq + kKv8Page) : a.max_ctx;
+  int splits = 1;
+  while (splits < kMaxCluster && pairs * splits * 2 <= (int64_t)a.sm_count * T::PER_SM && splits * 2 * kKeys <= keys) splits *= 2;
+  auto kern = a.alibi ? kv8_attn_kernel<HD, RT, true> : kv8_attn_kernel<HD, RT, false>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+  if (e == cudaSuccess && splits > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = dim3((unsigned)(row_tiles * splits), a.c.kv_heads, a.batch);
+  lc.blockDim = dim3(T::THREADS);
+  lc.dynamicSmemBytes = T::SMEM;
+  lc.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = splits;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  lc.attrs = at;
+  lc.numAttrs = splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&lc, kern, mk, mv, a, splits);
+}
+
+template <int HD> cudaError_t launch_hd(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.seq * (a.heads / a.c.kv_heads);
+  if (rows <= 8) return launch<HD, 8>(mk, mv, a, s);
+  if (rows <= 16) return launch<HD, 16>(mk, mv, a, s);
+  if (rows <= 32) return launch<HD, 32>(mk, mv, a, s);
+  return launch<HD, 64>(mk, mv, a, s);
+}
+
+}  // namespace
+
+bool kv8_attention_tc_supported(const Kv8AttnArgs& a) {
+  const auto low4 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; };
+  return (a.c.head_dim == 64 || a.c.head_dim == 128) && !low4(a.c.k) && !low4(a.c.v) && !low4(a.c.k_scale) &&
+         !low4(a.c.v_scale) && (int64_t)a.c.pages * a.c.kv_heads * kKv8Page <= INT_MAX;
+}
+
+cudaError_t kv8_attention_tc(const Kv8AttnArgs& a, cudaStream_t s) {
+  alignas(64) CUtensorMap mk, mv;
+  const int hd = a.c.head_dim;
+  const int sw = hd == 128 ? (int)CU_TENSOR_MAP_SWIZZLE_128B : (int)CU_TENSOR_MAP_SWIZZLE_64B;
+  const uint64_t rows = (uint64_t)a.c.pages * a.c.kv_heads * kKv8Page;
+  if (!make_tma_2d(&mk, a.c.k, (int)CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, hd, rows, hd, hd, kKv8Page, sw) ||
+      !make_tma_2d(&mv, a.c.v, (int)CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, hd, rows, hd, hd, kKv8Page, sw))
+    return cudaErrorInvalidValue;
+  return hd == 64 ? launch_hd<64>(mk, mv, a, s) : launch_hd<128>(mk, mv, a, s);
+}
+
+}  // namespace wv
