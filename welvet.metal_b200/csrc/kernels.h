@@ -294,7 +294,7 @@ cudaError_t kv_append(const void* k, const void* v, int ld, int rows, int kd, in
 
 // ---- per-head q/k norm with the position rotation (qk_norm.cu)
 constexpr int kQkNormMaxHeadDim = 512;
-constexpr int kQkNormParts = 592;  // most rows of the gamma-gradient partials (4 CTAs per SM)
+constexpr int kQkNormParts = 592;  // most CTAs of the backward (4 on each of 148 SMs): gamma-gradient partials
 struct QkNormArgs {
   int64_t tokens = 0;
   int heads = 0, kv_heads = 0, head_dim = 0;  // head_dim even, at most kQkNormMaxHeadDim
@@ -320,7 +320,6 @@ struct QkNormArgs {
   float* dq_gamma = nullptr;
   float* dk_gamma = nullptr;
   float* partial = nullptr;        // qk_norm_workspace_bytes(head_dim)
-  int part_q = 0;                  // set by qk_norm_backward
   uint32_t* err = nullptr;
   int sm_count = 148;
 };

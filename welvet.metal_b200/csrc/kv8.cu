@@ -92,6 +92,128 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const Kv8AppendArgs a) 
   if (threadIdx.x == 0) *scale = s;
 }
 
+// head_dim 64 and 128, 16-byte aligned rows, codes and table: one warp per (block, KV
+// head, K or V) holds the block's 16 rows in registers, 8 pairs of a row per lane (16
+// bytes of each half, the partners of the rotation together), so the rows are read
+// once and the maximum needs five shuffles. Bound by HBM for prompts (4 bytes read, 2
+// written a value pair of K and V), by latency for single tokens.
+constexpr int kAppendWarps = 8;
+template <int HD>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_vec_kernel(const Kv8AppendArgs a, int blocks) {
+  constexpr int LPR = HD / 16, RPW = 32 / LPR, IT = kKv8Block / RPW;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = (int)lane_id(), sub = lane / LPR, at = (lane % LPR) * 8;
+  int64_t unit = (int64_t)blockIdx.x * kAppendWarps + warp_id();
+  const int kh = (int)(unit % a.c.kv_heads);  // neighbouring warps read neighbouring heads of the same rows
+  unit /= a.c.kv_heads;
+  const bool is_v = (unit & 1) != 0;
+  unit >>= 1;
+  const int b = (int)(unit / blocks);
+  if (b >= a.batch) return;
+  const int n = kv8_new(a.seq_lens, b, a.seq), ctx = a.c.ctx_len[b], start = ctx - n;
+  const int first = max(start, 0), blk = first / kKv8Block + (int)(unit % blocks);
+  const int p0 = blk * kKv8Block, lo = max(first, p0), hi = min(ctx, p0 + kKv8Block);
+  if (lo >= hi) return;
+  const int page = kv8_page(a.c, b, blk / kKv8Subs, a.err);
+  if (page < 0) return;
+  const size_t ph = (size_t)page * a.c.kv_heads + kh;
+  uint8_t* codes = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + (ph * kKv8Page + p0 % kKv8Page) * HD + at;
+  float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + ph * kKv8Subs + blk % kKv8Subs;
+  const int ld = is_v ? a.ldv : a.ldk;
+  const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(is_v ? a.v : a.k) + (size_t)kh * HD + at;
+  const float s_old = lo > p0 ? *scale : 0.f;
+
+  uint4 raw[IT][2];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int p = p0 + it * RPW + sub;
+    raw[it][0] = raw[it][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (p < lo || p >= hi) continue;
+    const __nv_bfloat16* x = src + ((size_t)b * a.seq + (p - start)) * ld;
+    raw[it][0] = *reinterpret_cast<const uint4*>(x);
+    raw[it][1] = *reinterpret_cast<const uint4*>(x + HD / 2);
+  }
+  float x[IT][2][8], amax = 0.f;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int p = p0 + it * RPW + sub;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const uint32_t w[4] = {raw[it][hf].x, raw[it][hf].y, raw[it][hf].z, raw[it][hf].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[it][hf][2 * i] = __uint_as_float(w[i] << 16);
+        x[it][hf][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+    if (!is_v && a.rope && p >= lo && p < hi) {
+      if (p < a.max_pos) {
+        const float4* tab = reinterpret_cast<const float4*>(a.rope + (size_t)p * (HD / 2) + at);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float4 c = tab[i / 2];
+          const float cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float u = x[it][0][i + e], w = x[it][1][i + e];
+            x[it][0][i + e] = __fsub_rn(__fmul_rn(u, cs[2 * e]), __fmul_rn(w, cs[2 * e + 1]));
+            x[it][1][i + e] = __fadd_rn(__fmul_rn(u, cs[2 * e + 1]), __fmul_rn(w, cs[2 * e]));
+          }
+        }
+      } else if (a.err) {
+        atomicCAS(a.err, 0u, kErrRopePos);
+      }
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float m = fabsf(x[it][hf][i]);
+        amax = fmaxf(amax, m < INFINITY ? m : INFINITY);  // NaN counts as infinite
+      }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const bool poison = amax == INFINITY || s_old != s_old;
+  const float s = poison ? __uint_as_float(0x7fc00000u) : fmaxf(kv8_scale(amax), s_old);
+  // s is a power of two between 2^-64 and 2^120 (or the caller's own larger scale):
+  // multiplying by 1/s is dividing by s.
+  const float inv = poison ? 0.f : 1.f / s;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int r = it * RPW + sub, p = p0 + r;
+    if (p < lo || p >= hi) continue;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      uint32_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = poison ? 0u : e4m3x2(x[it][hf][2 * i] * inv, x[it][hf][2 * i + 1] * inv);
+      *reinterpret_cast<uint2*>(codes + (size_t)r * HD + hf * (HD / 2)) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    }
+  }
+  if (lo > p0) {
+    if (!poison && s != s_old) {  // the held codes move to the larger scale
+      const float f = s_old * inv;
+      for (int r = sub; r < lo - p0; r += RPW)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint2* q = reinterpret_cast<uint2*>(codes + (size_t)r * HD + hf * (HD / 2));
+          const uint32_t w[2] = {q->x, q->y};
+          uint32_t o[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 y = e4m3x2_value(w[i] & 0xffffu), z = e4m3x2_value(w[i] >> 16);
+            o[i] = e4m3x2(y.x * f, y.y * f) | (e4m3x2(z.x * f, z.y * f) << 16);
+          }
+          *q = make_uint2(o[0], o[1]);
+        }
+    }
+    __syncwarp();  // every lane has read the old scale
+  }
+  if (lane == 0) *scale = s;
+}
+
 // --------------------------------------------------------- attention, any shape
 constexpr int kGenWarps = 4;
 
@@ -186,6 +308,12 @@ __global__ void __launch_bounds__(kGenWarps * 32) kv8_attn_rows_kernel(const Kv8
 cudaError_t kv8_append(const Kv8AppendArgs& a, cudaStream_t s) {
   // blocks that seq tokens can touch, wherever they begin
   const int blocks = (a.seq + kKv8Block - 2) / kKv8Block + 1;
+  const auto low = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+  const int64_t ctas = ((int64_t)blocks * 2 * a.c.kv_heads * a.batch + kAppendWarps - 1) / kAppendWarps;
+  if ((a.c.head_dim == 64 || a.c.head_dim == 128) && a.ldk % 8 == 0 && a.ldv % 8 == 0 && !low(a.k) && !low(a.v) &&
+      !low(a.c.k) && !low(a.c.v) && !low(a.rope) && ctas < (1ll << 31))
+    return launch_pdl(a.c.head_dim == 64 ? kv8_append_vec_kernel<64> : kv8_append_vec_kernel<128>, dim3((unsigned)ctas),
+                      dim3(kAppendWarps * 32), 0, s, a, blocks);
   return launch_pdl(kv8_append_kernel, dim3(blocks, 2 * a.c.kv_heads, a.batch), dim3(128), 0, s, a);
 }
 
