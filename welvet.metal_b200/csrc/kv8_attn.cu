@@ -9,25 +9,27 @@
 // pass over the keys, so a decode step needs a 16-column MMA and no padding of queries
 // to 128 rows, and a thread of the softmax holds one key of every column: no work is
 // spent on absent queries, and no row reductions across lanes are needed per tile.
-// What the small operands lose in 8 bits is kept in more columns (columns are nearly
-// free while the 128-row operand sets the pace):
-//   * a query row, scaled by a power of two to at most 448, is hi + lo/16, two E4M3
-//     codes: exact to 2^-14 or better of 448, i.e. BF16 queries to 2^-22 of the row's
-//     largest value;
-//   * a probability is hi + lo/8 + lo2/64, three E5M2 codes (3 significant bits each,
-//     rounded to nearest in turn): a relative 2^-10, down to 2^-28 of the largest
+// What the small operands lose in 8 bits is kept in more of them:
+//   * a query row, scaled by a power of two to at most 448, is a sum of two E4M3 codes:
+//     exact to 2^-10 of 448, i.e. BF16 queries to 2^-19 of the row's largest value;
+//   * a probability, rounded to FP16, is a sum of three E5M2 codes (3 significant bits
+//     each, rounded to nearest in turn): a relative 2^-9, down to 2^-28 of the largest
 //     before the codes run out, so that long tails of small probabilities still add
-//     up. E4M3 codes would be finer but end at 2^-16 of the largest.
+//     up. E4M3 codes would be finer but end at 2^-20 of the largest.
+// The codes of one sum are columns side by side (2 RT of S, 3 RT of O), added when
+// read: a 128-row MMA of 32 bytes takes about 60 cycles for any N up to 128, so one
+// wide MMA is cheaper than several narrow ones into the same columns.
 // Scores and sums are FP32 (TMEM accumulators, registers).
 //
 // Softmax in the log2 domain with the value scale folded in: z = s kscale qscale
 // scale log2e + log2(vscale), p = 2^(z - ref), O += p * code, l += p / vscale. ref is a
-// column's running maximum of z, raised only when some z exceeds it by more than 2^8
+// column's running maximum of z, raised only when some z exceeds it by more than 2^4
 // (E5M2 has the room), so that most tiles need one vote and no maximum at all; when
-// it moves, the CTA's O and l are rescaled.
+// it moves, O and l are rescaled.
 //
-// Roles: one or two softmax warpgroups (a column group each; thread = TMEM lane =
-// key), a TMA warp (pages of codes and their four scales into a ring of 128-key
+// Roles: softmax warpgroups (thread = TMEM lane = key; NCG column groups share a tile,
+// NTG tile groups take tiles in turn with an O, ref and l of their own, joined at the
+// end), a TMA warp (pages of codes and their four scales into a ring of 128-key
 // stages), an MMA warp (S_0, S_1, then PV_i, S_{i+2}; S and P double-buffered).
 // A long context is split over a cluster of up to 16 CTAs whose partial (ref, l, O)
 // are joined through distributed shared memory in rank order: no workspace, no second
@@ -46,42 +48,53 @@ namespace wv {
 namespace {
 
 constexpr int kKeys = 128;          // keys of a tile: two pages
-constexpr float kBias = 6.f;        // log2 of p at the reference
-constexpr float kSlack = 8.f;       // z may exceed the reference by this much
+constexpr float kBias = 11.f;       // log2 of p at the reference
+constexpr float kSlack = 4.f;       // z may exceed the reference by this much (p <= 2^15)
 constexpr float kNoRef = 1e30f;     // bias - ref of a column that has seen no key
 constexpr int kMaxCluster = 16;
 
+// Column and tile groups: enough softmax warps to hide the latency of a tile's chain
+// (MMA, TMEM load, exponentials, conversion, store, MMA) within the registers.
 template <int HD, int RT> struct KT {
-  static constexpr int NWG = RT > 16 ? 2 : 1;       // softmax warpgroups
-  static constexpr int CPW = RT / NWG;              // columns of one
-  static constexpr int THREADS = NWG * 128 + 64;
+  static constexpr int NCG = RT == 64 ? 4 : RT == 32 ? 2 : 1;
+  static constexpr int NTG = RT == 64 || (RT == 32 && HD == 64) ? 1 : 2;
+  static constexpr int CPW = RT / NCG;              // columns of a warpgroup
+  static constexpr int SOFT_WARPS = NCG * NTG * 4;
+  static constexpr int THREADS = SOFT_WARPS * 32 + 64;
   static constexpr int TILE = kKeys * HD;           // bytes of a K or V tile
   static constexpr int STAGE = 2 * TILE;
-  // 512 TMEM columns (RT = 64) take the SM for one CTA; the deeper ring then takes its
-  // shared memory too, so that no other CTA of these kernels waits there for columns.
-  static constexpr int STAGES = (HD == 64 ? 4 : 3) + (RT == 64 ? (HD == 64 ? 4 : 1) : 0);
   static constexpr int NS = 2 * RT;                 // columns of S: hi | lo
-  static constexpr int NP = RT == 8 ? 32 : 3 * RT;  // columns of P and O: hi | lo | lo2
-  static constexpr int P_BYTES = kKeys * NP;
+  static constexpr int NO = RT == 8 ? 32 : 3 * RT;  // columns of O and P: three terms
+  static constexpr int O_COL = 2 * NS;              // TMEM: S_0 | S_1 | O of the tile groups
+  static constexpr int COLS = O_COL + NTG * NO;
+  static constexpr int TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr int STAGES = TMEM < 512 ? (HD == 64 ? 4 : 3) : (HD == 64 ? 8 : 4);
+  static constexpr int P_BYTES = kKeys * NO;
   static constexpr int Q_BYTES = NS * HD;
-  static constexpr int TMEM = RT == 8 ? 64 : RT == 16 ? 128 : RT == 32 ? 256 : 512;
-  static constexpr int O_COL = 2 * NS;              // TMEM: S_0 | S_1 | O
   static constexpr int OFF_P = STAGES * STAGE;
   static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
-  static constexpr int OFF_SC = OFF_Q + Q_BYTES;    // scales: [stage][K, V][8]
-  static constexpr int OFF_COL = OFF_SC + STAGES * 64;  // per column: (factor, bias - ref)
-  static constexpr int OFF_QHI = OFF_COL + RT * 8;      // last key of a column
+  static constexpr int OFF_SC = OFF_Q + Q_BYTES;          // scales: [stage][K, V][8]
+  static constexpr int OFF_OUT = OFF_SC + STAGES * 64;    // output element of a column (64 bits), -1: none
+  static constexpr int OFF_QF = OFF_OUT + RT * 8;         // factor of a column's scores
+  static constexpr int OFF_REF = OFF_QF + RT * 4;         // [NTG][RT] bias - reference
+  static constexpr int OFF_FAC = OFF_REF + NTG * RT * 4;  // [NTG][RT] rescaling factors
+  static constexpr int OFF_L = OFF_FAC + NTG * RT * 4;    // [NTG][RT] sums
+  static constexpr int OFF_QHI = OFF_L + NTG * RT * 4;    // last key of a column
   static constexpr int OFF_SLOPE = OFF_QHI + RT * 4;
-  static constexpr int OFF_L = OFF_SLOPE + RT * 4;      // sums of the CTA
-  static constexpr int OFF_RED = OFF_L + RT * 4;        // [4 warps][RT]
-  static constexpr int OFF_BAR = OFF_RED + 4 * RT * 4;
-  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (2 * STAGES + 6) + 32;
+  static constexpr int OFF_RED = OFF_SLOPE + RT * 4;      // [NTG][4 warps][RT]
+  static constexpr int OFF_BAR = OFF_RED + NTG * 4 * RT * 4;
+  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (2 * STAGES + 7) + 32;
   // resident CTAs of an SM
   static constexpr int BY_SMEM = 228 * 1024 / (SMEM + 1024), BY_TMEM = 512 / TMEM;
   static constexpr int PER_SM = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
-  // Partial O of a split, [RT][HD] FP32, over the stages once every MMA has read them.
-  static_assert(RT * HD * 4 <= STAGES * STAGE, "partial outputs over the stages");
-  static_assert(O_COL + NP <= TMEM, "TMEM columns");
+  // A CTA that waits for TMEM columns while its cluster waits for it could wait for a
+  // CTA of another stream in the same state. Shared memory rules that out: the CTAs of
+  // these kernels that fit an SM together never need more than its 512 columns.
+  static_assert(SMEM > 72 * 1024 && (TMEM < 512 || SMEM > (228 - 72) * 1024), "TMEM columns of co-resident CTAs");
+  // Partial O, [RT][HD] FP32, over the stages, and the cluster's [16][RT] references,
+  // sums and weights over P, once every MMA has read them.
+  static_assert(RT * HD * 4 <= STAGES * STAGE && 3 * 16 * RT * 4 <= 2 * P_BYTES, "joining areas");
+  static_assert(COLS <= TMEM, "TMEM columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -151,21 +164,34 @@ template <int ID> WV_DEV bool bar_any(bool v) {
   return r != 0;
 }
 template <int ID> WV_DEV void bar_sync() { asm volatile("barrier.cta.sync %0, 128;" ::"n"(ID) : "memory"); }
-template <int NWG> WV_DEV bool wg_any(int wg, bool v) { return NWG == 1 || wg == 0 ? bar_any<1>(v) : bar_any<2>(v); }
-template <int NWG> WV_DEV void wg_sync(int wg) {
-  if (NWG == 1 || wg == 0) bar_sync<1>();
-  else bar_sync<2>();
+// ... of warpgroup w of N (barrier 0 is the CTA's).
+template <int N> WV_DEV bool wg_any(int w, bool v) {
+  if (N == 1 || w == 0) return bar_any<1>(v);
+  if (N == 2 || w == 1) return bar_any<2>(v);
+  return w == 2 ? bar_any<3>(v) : bar_any<4>(v);
 }
-// Two FP32 values as E5M2 codes (nearest, saturating), and the values of two codes: an
-// E5M2 code is the upper byte of the FP16 pattern of its value.
-WV_DEV uint32_t e5m2x2(float lo, float hi) {
+template <int N> WV_DEV void wg_sync(int w) {
+  if (N == 1 || w == 0) bar_sync<1>();
+  else if (N == 2 || w == 1) bar_sync<2>();
+  else if (w == 2) bar_sync<3>();
+  else bar_sync<4>();
+}
+template <int WARPS> WV_DEV void soft_sync() { asm volatile("barrier.cta.sync 5, %0;" ::"n"(WARPS * 32) : "memory"); }
+// FP16 pairs to E5M2 codes (nearest), and the FP16 values of two codes: an E5M2 code is
+// the upper byte of the FP16 pattern of its value.
+WV_DEV uint32_t e5m2x2(__half2 v) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&v)));
   return r;
 }
-WV_DEV float2 e5m2x2_value(uint32_t c) {
+WV_DEV __half2 e5m2x2_value(uint32_t c) {
   const uint32_t h = __byte_perm(c, 0u, 0x1404);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return *reinterpret_cast<const __half2*>(&h);
+}
+WV_DEV uint64_t fmul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 WV_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -189,7 +215,7 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const Kv8AttnArgs a, int splits) {
   using T = KT<HD, RT>;
-  constexpr int CPW = T::CPW, ST = T::STAGES;
+  constexpr int CPW = T::CPW, ST = T::STAGES, NTG = T::NTG, NCG = T::NCG, kSoftWarps = T::SOFT_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::OFF_BAR);
@@ -197,15 +223,17 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   uint64_t* s_full = empty + ST;  // [2]
   uint64_t* p_full = s_full + 2;  // [2]
   uint64_t* pv_done = p_full + 2; // [2]
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pv_done + 2);
+  uint64_t* q_full = pv_done + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  float2* col = reinterpret_cast<float2*>(smem + T::OFF_COL);
+  int64_t* outs = reinterpret_cast<int64_t*>(smem + T::OFF_OUT);
+  float* qf = reinterpret_cast<float*>(smem + T::OFF_QF);
+  float* refs = reinterpret_cast<float*>(smem + T::OFF_REF);
+  float* facs = reinterpret_cast<float*>(smem + T::OFF_FAC);
+  float* lsum = reinterpret_cast<float*>(smem + T::OFF_L);
   int* qhi = reinterpret_cast<int*>(smem + T::OFF_QHI);
   float* slope = reinterpret_cast<float*>(smem + T::OFF_SLOPE);
-  float* lsum = reinterpret_cast<float*>(smem + T::OFF_L);
-  float* red = reinterpret_cast<float*>(smem + T::OFF_RED);
   const int warp = (int)warp_id(), lane = (int)lane_id();
-  constexpr int kSoftWarps = T::NWG * 4;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -214,9 +242,10 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kSoftWarps);
+      mbar_init(&p_full[i], NCG * 4);  // the warps that share a tile
       mbar_init(&pv_done[i], 1);
     }
+    mbar_init(q_full, kSoftWarps);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -224,15 +253,19 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     tmem_alloc(tmem_holder, T::TMEM);
     tmem_relinquish();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
   pdl_wait();  // the append (or whatever filled the cache, q and the lengths) is complete
+  pdl_trigger();  // behind the TMEM allocation: a dependent's CTA must not take the columns first
 
   // ---- this CTA's columns and keys
   const int split = blockIdx.x % splits, b = blockIdx.z;
   const int kh = blockIdx.y, r0 = (int)(blockIdx.x / splits) * RT;
   const int G = a.heads / a.c.kv_heads;
   const int n = kv8_new(a.seq_lens, b, a.seq);
-  int ctx = a.c.ctx_len[b];
-  const int shift = ctx - n;  // position of the first new token
+  const int shift = a.c.ctx_len[b] - n;  // position of the first new token
   const int t0 = max(r0 / G, max(0, -shift)), t1 = min((r0 + RT - 1) / G, n - 1);  // live tokens
   const int qlo = shift + t0;
   int k1 = t1 >= t0 ? shift + t1 + 1 : 0;
@@ -245,49 +278,7 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   const int per = (all + splits - 1) / splits;
   const int tile0 = min(all, split * per), tiles = min(all, tile0 + per) - tile0;
   const int base0 = page0 * kKv8Page + tile0 * kKeys;  // first key of tile 0
-
-  // ---- queries: hi and lo codes, [16-byte chunk of hd][2 RT rows][16]
-  if (warp < kSoftWarps) {
-    for (int c = warp; c < RT; c += kSoftWarps) {
-      const int t = (r0 + c) / G, h = kh * G + (r0 + c) % G;
-      const bool live = t >= t0 && t <= t1;
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + t) * a.ldq + (size_t)h * HD;
-      float x[HD / 32], m = 0.f;
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        x[i] = live ? __bfloat162float(q[lane + 32 * i]) : 0.f;
-        m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
-      }
-      m = warp_max(m);
-      const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
-      const float s = bad ? 1.f : kv8_scale(m);
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const int e = lane + 32 * i;
-        const float y = bad ? 0.f : x[i] / s;
-        const uint32_t hi = e4m3x2(y, 0.f);
-        const uint32_t lo = e4m3x2((y - e4m3x2_value(hi).x) * 16.f, 0.f);
-        uint8_t* dst = smem + T::OFF_Q + (e / 16) * (T::NS * 16) + e % 16;
-        dst[c * 16] = (uint8_t)hi;
-        dst[(RT + c) * 16] = (uint8_t)lo;
-      }
-      if (lane == 0) {
-        col[c] = make_float2(bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e, kNoRef);
-        qhi[c] = live ? min(shift + t, k1 - 1) : k1 - 1;  // a column without a query sees whatever there is
-        if (ALIBI) slope[c] = exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * kLog2e;
-      }
-    }
-    fence_proxy_async_smem();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
-  pdl_trigger();  // behind the TMEM allocation: a dependent's CTA must not take the columns first
   bool ok = true;
-  float l[CPW];
-#pragma unroll
-  for (int c = 0; c < CPW; ++c) l[c] = 0.f;
 
   if (warp == kSoftWarps) {
     // ------------------------------------------------------------- TMA producer
@@ -326,74 +317,130 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
         mbar_arrive_expect_tx(&full[s], two * (2 * kKv8Page * HD + 32));
         for (int i = 0; i < two; ++i) {
           const int ph = id[i] * a.c.kv_heads + kh;
-          tma_load_2d(kt + i * kKv8Page * HD, &tmK, &full[s], 0, ph * kKv8Page);
           bulk_load(sc + i * 4, a.c.k_scale + (size_t)ph * kKv8Subs, 16, &full[s]);
-          tma_load_2d(kt + T::TILE + i * kKv8Page * HD, &tmV, &full[s], 0, ph * kKv8Page);
           bulk_load(sc + 8 + i * 4, a.c.v_scale + (size_t)ph * kKv8Subs, 16, &full[s]);
+          tma_load_2d(kt + i * kKv8Page * HD, &tmK, &full[s], 0, ph * kKv8Page);
+          tma_load_2d(kt + T::TILE + i * kKv8Page * HD, &tmV, &full[s], 0, ph * kKv8Page);
         }
       }
     }
   } else if (warp == kSoftWarps + 1) {
     // --------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t kRow = HD == 128 ? 2u : 4u;  // swizzle of the code tiles
-      constexpr uint32_t HI_KV = desc_hi(8 * HD, kRow);       // 8 keys of HD bytes
-      constexpr uint32_t HI_Q = desc_hi(128, 0);              // 8 rows of 16 bytes
-      constexpr uint32_t HI_P = desc_hi(kKeys * 16, 0);       // 16 columns of every key
-      constexpr uint32_t IDESC_S = idesc_f8(0, 0, 128, T::NS, 0, 0);
-      constexpr uint32_t IDESC_PV = idesc_f8(0, 1, HD, T::NP, 1, 1);
-      const uint32_t q_lo = sdesc_lo(smem_u32(smem + T::OFF_Q), T::NS * 16);
-      auto issue_s = [&](int j) -> bool {
-        const int s = j % ST;
-        if (!mbar_wait(&full[s], (j / ST) & 1, abort_flag, a.err, kErrWaitFull)) return false;
-        tc_fence_after();
-        const uint32_t k_lo = sdesc_lo(smem_u32(smem + s * T::STAGE), 16);
+    // The whole warp walks the loop (descriptors stay warp-uniform), one lane issues.
+    constexpr uint32_t kRow = HD == 128 ? 2u : 4u;  // swizzle of the code tiles
+    constexpr uint32_t HI_KV = desc_hi(8 * HD, kRow);       // 8 keys of HD bytes
+    constexpr uint32_t HI_Q = desc_hi(128, 0);              // 8 rows of 16 bytes
+    constexpr uint32_t HI_P = desc_hi(kKeys * 16, 0);       // 16 columns of every key
+    constexpr uint32_t IDESC_S = idesc_f8(0, 0, 128, T::NS, 0, 0);
+    constexpr uint32_t IDESC_PV = idesc_f8(0, 1, HD, T::NO, 1, 1);
+    const uint32_t base = smem_u32(smem);
+    const uint32_t q_lo = sdesc_lo(base + T::OFF_Q, T::NS * 16);
+    const bool lead = elect_one();
+    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.err, code)) != 0;
+    };
+    auto issue_s = [&](int j) -> bool {
+      const int s = j % ST;
+      if (!wait(&full[s], (j / ST) & 1, kErrWaitFull)) return false;
+      tc_fence_after();
+      const uint32_t k_lo = sdesc_lo(base + s * T::STAGE, 16);
+      if (lead) {
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk)
           umma_f8(tmem + (uint32_t)((j & 1) * T::NS), k_lo + kk * 2, HI_KV, q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
         umma_commit(&s_full[j & 1]);
-        return true;
-      };
-      for (int j = 0; ok && j < min(2, tiles); ++j) ok = issue_s(j);
-      for (int i = 0; ok && i < tiles; ++i) {
-        ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitOther);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t v_lo = sdesc_lo(smem_u32(smem + (i % ST) * T::STAGE + T::TILE), 16);
-        const uint32_t p_lo = sdesc_lo(smem_u32(smem + T::OFF_P + (i & 1) * T::P_BYTES), 128);
+      }
+      __syncwarp();
+      return true;
+    };
+    if (tiles > 0) ok = wait(q_full, 0, kErrWaitOther);
+    for (int j = 0; ok && j < min(2, tiles); ++j) ok = issue_s(j);
+    for (int i = 0; ok && i < tiles; ++i) {
+      ok = wait(&p_full[i & 1], (i >> 1) & 1, kErrWaitOther);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t v_lo = sdesc_lo(base + (i % ST) * T::STAGE + T::TILE, 16);
+      const uint32_t p_lo = sdesc_lo(base + T::OFF_P + (i & 1) * T::P_BYTES, 128);
+      const uint32_t first = i >= NTG ? 1u : 0u;
+      if (lead) {
 #pragma unroll
         for (int kk = 0; kk < kKeys / 32; ++kk)
-          umma_f8(tmem + T::O_COL, v_lo + kk * (32 * HD / 16), HI_KV, p_lo + kk * (32 * 16 / 16), HI_P, IDESC_PV,
-                  (i > 0 || kk > 0) ? 1u : 0u);
+          umma_f8(tmem + T::O_COL + (i % NTG) * T::NO, v_lo + kk * (32 * HD / 16), HI_KV, p_lo + kk * 32, HI_P, IDESC_PV,
+                  kk > 0 ? 1u : first);
         umma_commit(&empty[i % ST]);
         umma_commit(&pv_done[i & 1]);
-        if (i + 2 < tiles) ok = issue_s(i + 2);
       }
+      __syncwarp();
+      if (i + 2 < tiles) ok = issue_s(i + 2);
     }
   } else {
+    // ---- queries: hi and lo codes, [16-byte chunk of hd][RT hi rows, RT lo rows][16]
+    for (int c = warp; c < RT; c += kSoftWarps) {
+      const int t = (r0 + c) / G, h = kh * G + (r0 + c) - t * G;
+      const bool live = t >= t0 && t <= t1;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + t) * a.ldq + (size_t)h * HD;
+      float x[HD / 32], m = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        x[i] = live ? __bfloat162float(q[lane + 32 * i]) : 0.f;
+        m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
+      }
+      m = warp_max(m);
+      const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
+      const float s = bad ? 1.f : kv8_scale(m);
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const int e = lane + 32 * i;
+        const float y = bad ? 0.f : x[i] / s;
+        const uint32_t hi = e4m3x2(y, 0.f);
+        const uint32_t lo = e4m3x2(y - e4m3x2_value(hi).x, 0.f);
+        uint8_t* dst = smem + T::OFF_Q + (e / 16) * (T::NS * 16) + e % 16;
+        dst[c * 16] = (uint8_t)hi;
+        dst[(RT + c) * 16] = (uint8_t)lo;
+      }
+      if (lane == 0) {
+        qf[c] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
+        for (int g = 0; g < NTG; ++g) refs[g * RT + c] = kNoRef;
+        // a column without a query sees whatever there is; its output is zero, or none
+        qhi[c] = live ? min(shift + t, k1 - 1) : k1 - 1;
+        outs[c] = t >= a.seq ? -1 : (((int64_t)b * a.seq + t) * a.ldo + (int64_t)h * HD) * 2 + (live ? 1 : 0);
+        if (ALIBI) slope[c] = exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * kLog2e;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    soft_sync<kSoftWarps>();
+
     // ------------------------------------------------------------------ softmax
-    const int wg = warp >> 2, w4 = warp & 3;
+    const int wg = warp >> 2, w4 = warp & 3, tg = wg / NCG, c0 = (wg % NCG) * CPW;
     const int key = 32 * w4 + lane;  // of the tile; this thread's TMEM lane
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16);
-    const int c0 = wg * CPW;
-    for (int i = 0; i < tiles; ++i) {
+    float* ref = refs + tg * RT + c0;
+    float* fac = facs + tg * RT + c0;
+    float* red = reinterpret_cast<float*>(smem + T::OFF_RED) + tg * 4 * RT + c0;
+    const auto pair = [](const float* p) { return *reinterpret_cast<const uint64_t*>(p); };
+    uint64_t l2[CPW / 2];  // sums of the columns, in pairs
+#pragma unroll
+    for (int c = 0; c < CPW / 2; ++c) l2[c] = 0ull;
+    for (int i = tg; i < tiles; i += NTG) {
       const int s = i % ST, base = base0 + i * kKeys, kpos = base + key;
       // After a wait that gave up, the tiles are still walked (the waits return at once):
       // the warpgroup's barriers need every thread.
-      ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
-      ok = mbar_wait(&full[s], (i / ST) & 1, abort_flag, a.err, kErrWaitFull) && ok;  // its scales
-      tc_fence_after();
+      ok = mbar_wait(&full[s], (i / ST) & 1, abort_flag, a.err, kErrWaitFull) && ok;  // the scales
       const float* sc = reinterpret_cast<const float*>(smem + T::OFF_SC + s * 64);
       const bool on = kpos < k1;
       const float ks = sc[key >> 4], vs = sc[8 + (key >> 4)];
-      float ev, inv;
+      float ev;
       asm("lg2.approx.f32 %0, %1;" : "=f"(ev) : "f"(vs));
-      inv = on && vs == vs ? __frcp_rn(vs) : 0.f;
-      if (!on && wg == 0) {  // rows past the context may hold NaN codes: 0 * NaN
+      const float inv = on && vs == vs ? __fdividef(1.f, vs) : 0.f;
+      if (!on && c0 == 0) {  // rows past the context may hold NaN codes: 0 * NaN
         uint8_t* row = smem + s * T::STAGE + T::TILE + key * HD;
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < HD; x += 16) *reinterpret_cast<uint4*>(row + x) = make_uint4(0u, 0u, 0u, 0u);
       }
+      ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
+      tc_fence_after();
       // z of this key for the group's columns
       float z[CPW];
       {
@@ -401,82 +448,95 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
         tmem_ld<CPW>(tl + (i & 1) * T::NS + c0, hi);
         tmem_ld<CPW>(tl + (i & 1) * T::NS + RT + c0, lo);
         tmem_ld_wait();
+        const uint64_t ks2 = f2pack(ks, ks), ev2 = f2pack(ev, ev);
 #pragma unroll
-        for (int c = 0; c < CPW; ++c)
-          z[c] = fmaf(fmaf(__uint_as_float(lo[c]), 0.0625f, __uint_as_float(hi[c])) * ks, col[c0 + c].x, ev);
+        for (int c = 0; c < CPW; c += 2) {
+          const uint64_t s2 = fadd2(f2pack(__uint_as_float(hi[c]), __uint_as_float(hi[c + 1])),
+                                    f2pack(__uint_as_float(lo[c]), __uint_as_float(lo[c + 1])));
+          f2unpack(ffma2(s2, fmul2(ks2, pair(qf + c0 + c)), ev2), z[c], z[c + 1]);
+        }
       }
       if (ALIBI) {
 #pragma unroll
         for (int c = 0; c < CPW; ++c) z[c] -= slope[c0 + c] * (float)(qhi[c0 + c] - kpos);
       }
-      if (base + kKeys > qlo + 1 || (a.window > 0 && base <= k1 - 1 - a.window)) {  // some column's edge
+      // some column's edge lies in the tile
+      if (base + kKeys > qlo + 1 || (a.window > 0 && base <= k1 - 1 - a.window)) {
+        const int w = a.window > 0 ? a.window : INT_MAX;
 #pragma unroll
-        for (int c = 0; c < CPW; ++c)
-          if (kpos > qhi[c0 + c] || (a.window > 0 && kpos <= qhi[c0 + c] - a.window)) z[c] = -INFINITY;
+        for (int c = 0; c < CPW; ++c) {
+          const int back = qhi[c0 + c] - kpos;
+          if (back < 0 || back >= w) z[c] = -INFINITY;
+        }
       }
-      bool high = false;
+      float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < CPW; ++c) high |= z[c] + col[c0 + c].y > kBias + kSlack;
-      if (i >= 2) ok = mbar_wait(&pv_done[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;  // P is free
-      if (wg_any<T::NWG>(wg, high)) {
+      for (int c = 0; c < CPW; c += 2) {
+        float u, w;
+        f2unpack(fadd2(f2pack(z[c], z[c + 1]), pair(ref + c)), u, w);
+        top = fmax3(top, u, w);
+      }
+      // P is free (and, with two tile groups, this group's O holds all its tiles)
+      if (i >= 2) ok = mbar_wait(&pv_done[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+      if (wg_any<NCG * NTG>(wg, top > kBias + kSlack)) {
         // new references: the maximum of every column over the tile's keys
 #pragma unroll
         for (int c = 0; c < CPW; ++c) {
           const float m = warp_max(z[c]);
-          if (lane == 0) red[w4 * RT + c0 + c] = m;
+          if (lane == 0) red[w4 * RT + c] = m;
         }
-        // O holds PV_{i-1}
-        if (i > 0) ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+        if (NTG == 1 && i > 0)
+          ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
         tc_fence_after();
-        wg_sync<T::NWG>(wg);
-        float f[CPW], ref[CPW];
-#pragma unroll
-        for (int c = 0; c < CPW; ++c) {
-          const int cc = c0 + c;
-          const float m = fmaxf(fmaxf(red[cc], red[RT + cc]), fmaxf(red[2 * RT + cc], red[3 * RT + cc]));
-          const float was = col[cc].y, now = m == -INFINITY ? was : fminf(was, kBias - m);
-          f[c] = was == kNoRef ? 1.f : fast_exp2(now - was);
-          ref[c] = now;
-          l[c] *= f[c];
+        wg_sync<NCG * NTG>(wg);
+        if (key < CPW) {
+          const float m = fmaxf(fmaxf(red[key], red[RT + key]), fmaxf(red[2 * RT + key], red[3 * RT + key]));
+          const float was = ref[key], now = m == -INFINITY ? was : fminf(was, kBias - m);
+          fac[key] = was == kNoRef ? 1.f : fast_exp2(now - was);
+          ref[key] = now;
         }
-        wg_sync<T::NWG>(wg);  // every thread has read the old references
+        wg_sync<NCG * NTG>(wg);
 #pragma unroll
-        for (int c = 0; c < CPW; ++c)
-          if (key == c) col[c0 + c].y = ref[c];
-        if (i > 0) {
-#pragma unroll
+        for (int c = 0; c < CPW; c += 2) l2[c / 2] = fmul2(l2[c / 2], pair(fac + c));
+        if (i >= NTG) {
+#pragma unroll 1
           for (int term = 0; term < 3; ++term) {
             uint32_t o[CPW];
-            tmem_ld<CPW>(tl + T::O_COL + term * RT + c0, o);
+            const uint32_t at = tl + T::O_COL + tg * T::NO + term * RT + c0;
+            tmem_ld<CPW>(at, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < CPW; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f[c]);
-            tmem_st<CPW>(tl + T::O_COL + term * RT + c0, o);
+            for (int c = 0; c < CPW; c += 2) {
+              float u, w;
+              f2unpack(fmul2(f2pack(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), pair(fac + c)), u, w);
+              o[c] = __float_as_uint(u);
+              o[c + 1] = __float_as_uint(w);
+            }
+            tmem_st<CPW>(at, o);
           }
           tmem_st_wait();
         }
-        wg_sync<T::NWG>(wg);  // the new references are in place
       }
       // probabilities, and their three codes: chunks of 16 columns (of 8 + 8 when RT = 8)
+      const uint64_t inv2 = f2pack(inv, inv);
       uint32_t code[3][CPW / 4];
 #pragma unroll
       for (int c = 0; c < CPW; c += 4) {
         float p[4];
+        f2unpack(fadd2(f2pack(z[c], z[c + 1]), pair(ref + c)), p[0], p[1]);
+        f2unpack(fadd2(f2pack(z[c + 2], z[c + 3]), pair(ref + c + 2)), p[2], p[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = fast_exp2(z[c + e] + col[c0 + c + e].y);
-          l[c + e] = fmaf(p[e], inv, l[c + e]);
-        }
+        for (int e = 0; e < 4; ++e) p[e] = fast_exp2(p[e]);
+        l2[c / 2] = ffma2(f2pack(p[0], p[1]), inv2, l2[c / 2]);
+        l2[c / 2 + 1] = ffma2(f2pack(p[2], p[3]), inv2, l2[c / 2 + 1]);
+        __half2 u = __floats2half2_rn(p[0], p[1]), w = __floats2half2_rn(p[2], p[3]);
 #pragma unroll
         for (int term = 0; term < 3; ++term) {
-          const uint32_t u = e5m2x2(p[0], p[1]), w = e5m2x2(p[2], p[3]);
-          code[term][c / 4] = u | (w << 16);
-          if (term < 2) {
-            const float2 x = e5m2x2_value(u), y = e5m2x2_value(w);
-            p[0] = (p[0] - x.x) * 8.f;
-            p[1] = (p[1] - x.y) * 8.f;
-            p[2] = (p[2] - y.x) * 8.f;
-            p[3] = (p[3] - y.y) * 8.f;
+          const uint32_t cu = e5m2x2(u), cw = e5m2x2(w);
+          code[term][c / 4] = cu | (cw << 16);
+          if (term < 2) {  // exact: the remainder has fewer bits than FP16 holds
+            u = __hsub2(u, e5m2x2_value(cu));
+            w = __hsub2(w, e5m2x2_value(cw));
           }
         }
       }
@@ -497,83 +557,115 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[i & 1]);
     }
-    if (tiles > 0)
-      ok = mbar_wait(&pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
-    tc_fence_after();
     // sums of the columns over the keys of the four warps, in warp order
 #pragma unroll
     for (int c = 0; c < CPW; ++c) {
-      float v = l[c];
+      float v, w;
+      f2unpack(l2[c / 2], v, w);
+      if (c & 1) v = w;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) red[w4 * RT + c0 + c] = v;
+      if (lane == 0) red[w4 * RT + c] = v;
     }
-    wg_sync<T::NWG>(wg);
-    if (key < CPW) lsum[c0 + key] = (red[c0 + key] + red[RT + c0 + key]) + (red[2 * RT + c0 + key] + red[3 * RT + c0 + key]);
+    wg_sync<NCG * NTG>(wg);
+    if (key < CPW) lsum[tg * RT + c0 + key] = (red[key] + red[RT + key]) + (red[2 * RT + key] + red[3 * RT + key]);
+    // every PV has completed (the last two cover the others: MMAs finish in order)
+    for (int i = max(0, tiles - 2); i < tiles; ++i)
+      ok = mbar_wait(&pv_done[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+    tc_fence_after();
+    soft_sync<kSoftWarps>();
+
+    // ---- O^T -> part [column][dim] over the stages; the tile groups are joined, in
+    // group order. From here on the code runs once, so it is kept short: fetching it
+    // costs more than running it.
+    if (threadIdx.x < RT) {
+      const int c = threadIdx.x;
+      float r = refs[c], den = lsum[c];
+      facs[c] = 1.f;
+      if constexpr (NTG == 2) {
+        r = fminf(r, refs[RT + c]);
+        const float f0 = fast_exp2(r - refs[c]), f1 = fast_exp2(r - refs[RT + c]);
+        facs[c] = f0;
+        facs[RT + c] = f1;
+        den = f0 * den + f1 * lsum[RT + c];
+      }
+      refs[c] = r;
+      // the weight of the CTA's own sums when the context is not split
+      lsum[c] = splits > 1 ? den : den == 0.f ? 0.f : 1.f / den;
+    }
+    soft_sync<kSoftWarps>();
+    float* part = reinterpret_cast<float*>(smem);
+    if (warp < NCG * 4) {
+      // lane = dim (head_dim 64: 16 lanes of every warp)
+      const int dim = HD == 128 ? 32 * w4 + lane : 16 * w4 + lane;
+#pragma unroll 1
+      for (int c = c0; c < c0 + CPW; c += 8) {
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll 1
+        for (int g = 0; g < min(NTG, tiles); ++g)
+#pragma unroll 1
+          for (int term = 0; term < 3; ++term) {
+            uint32_t x[8];
+            tmem_ld<8>(tl + T::O_COL + g * T::NO + term * RT + c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = fmaf(facs[g * RT + c + e], __uint_as_float(x[e]), o[e]);
+          }
+        if (HD == 128 || lane < 16) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) part[(c + e) * HD + dim] = o[e];
+        }
+      }
+    }
+    tc_fence_before();
   }
   // A bounded wait that gave up is in the error word: every thread still takes the
   // barriers below, and the outputs are not written.
   ok = __syncthreads_and(ok ? 1 : 0) != 0;
-
-  if (warp < kSoftWarps) {
-    // O^T: lane = dim (head_dim 64: 16 lanes of every warp), a column group per warpgroup
-    const int wg = warp >> 2, w4 = warp & 3, c0 = wg * CPW;
-    const int dim = HD == 128 ? 32 * w4 + lane : 16 * w4 + lane;
-    const bool mine = HD == 128 || lane < 16;
-    const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + T::O_COL + c0;
-    float o[CPW];
-    {
-      uint32_t x[CPW], y[CPW], w[CPW];
-      tmem_ld<CPW>(tl, x);
-      tmem_ld<CPW>(tl + RT, y);
-      tmem_ld<CPW>(tl + 2 * RT, w);
-      tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < CPW; ++c)
-        o[c] = tiles > 0 ? fmaf(fmaf(__uint_as_float(w[c]), 0.125f, __uint_as_float(y[c])), 0.125f, __uint_as_float(x[c])) : 0.f;
-    }
-    if (splits == 1) {
-      if (ok && mine) {
-#pragma unroll
-        for (int c = 0; c < CPW; ++c) {
-          const int r = r0 + c0 + c, t = r / G;
-          if (t >= a.seq) break;
-          const float den = lsum[c0 + c];
-          const bool live = t >= t0 && t <= t1;
-          static_cast<__nv_bfloat16*>(a.out)[((size_t)b * a.seq + t) * a.ldo + (size_t)(kh * G + r % G) * HD + dim] =
-              __float2bfloat16_rn(!live || den == 0.f ? 0.f : o[c] / den);
-        }
-      }
-    } else if (mine) {
-      float* part = reinterpret_cast<float*>(smem);
-#pragma unroll
-      for (int c = 0; c < CPW; ++c) part[(c0 + c) * HD + dim] = o[c];
-    }
-  }
-  if (splits > 1) {
-    cluster_sync();
-    // joined in rank order: 2^(ref_s - ref) of every split's O and l, (column, dim)
-    // pairs dealt out over the cluster
-    for (int idx = split * T::THREADS + threadIdx.x; idx < RT * HD; idx += splits * T::THREADS) {
-      const int c = idx / HD, r = r0 + c, t = r / G;
-      if (t >= a.seq) break;
-      float ref = kNoRef, num = 0.f, den = 0.f;
-      for (int s = 0; s < splits; ++s) ref = fminf(ref, ld_peer(peer_addr(&col[c].y, s)));
-      for (int s = 0; s < splits; ++s) {
-        const float f = fast_exp2(ref - ld_peer(peer_addr(&col[c].y, s)));
-        num = fmaf(f, ld_peer(peer_addr(reinterpret_cast<float*>(smem) + idx, s)), num);
-        den = fmaf(f, ld_peer(peer_addr(&lsum[c], s)), den);
-      }
-      const bool live = t >= t0 && t <= t1;
-      if (ok)
-        static_cast<__nv_bfloat16*>(a.out)[((size_t)b * a.seq + t) * a.ldo + (size_t)(kh * G + r % G) * HD + idx % HD] =
-            __float2bfloat16_rn(!live || den == 0.f ? 0.f : num / den);
-    }
-    cluster_sync();  // no CTA leaves while another reads its partials
-  }
-  tc_fence_before();
-  __syncthreads();
   if (warp == kSoftWarps) tmem_dealloc(tmem, T::TMEM);
+
+  float* part = reinterpret_cast<float*>(smem);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
+  if (splits == 1) {
+    for (int idx = threadIdx.x; ok && idx < RT * HD; idx += T::THREADS) {
+      const int c = idx / HD;
+      const int64_t to = outs[c];
+      if (to < 0) break;
+      out[(to >> 1) + idx % HD] = __float2bfloat16_rn(to & 1 ? part[idx] * lsum[c] : 0.f);
+    }
+    return;
+  }
+  // ---- the splits of a context are joined in rank order: 2^(ref_s - ref) of every
+  // split's O and l; (column, dim) pairs are dealt out over the cluster.
+  float* pr = reinterpret_cast<float*>(smem + T::OFF_P);  // [split][RT] references
+  float* pl = pr + kMaxCluster * RT;                      // sums
+  float* pw = pl + kMaxCluster * RT;                      // weights
+  cluster_sync();
+  for (int i = threadIdx.x; i < splits * RT; i += T::THREADS) {
+    pr[i] = ld_peer(peer_addr(&refs[i % RT], i / RT));
+    pl[i] = ld_peer(peer_addr(&lsum[i % RT], i / RT));
+  }
+  __syncthreads();
+  if (threadIdx.x < RT) {
+    float r = kNoRef, den = 0.f;
+    for (int s = 0; s < splits; ++s) r = fminf(r, pr[s * RT + threadIdx.x]);
+    for (int s = 0; s < splits; ++s) den = fmaf(fast_exp2(r - pr[s * RT + threadIdx.x]), pl[s * RT + threadIdx.x], den);
+    for (int s = 0; s < splits; ++s)
+      pw[s * RT + threadIdx.x] = den == 0.f ? 0.f : fast_exp2(r - pr[s * RT + threadIdx.x]) / den;
+  }
+  __syncthreads();
+  for (int idx = split * T::THREADS + threadIdx.x; ok && idx < RT * HD; idx += splits * T::THREADS) {
+    const int c = idx / HD;
+    const int64_t to = outs[c];
+    if (to < 0) break;
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) v = fmaf(pw[s * RT + c], ld_peer(peer_addr(part + idx, s)), v);
+    out[(to >> 1) + idx % HD] = __float2bfloat16_rn(to & 1 ? v : 0.f);
+  }
+  cluster_sync();  // no CTA leaves while another reads its partials
 }
 
 template <int HD, int RT> cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {

@@ -224,14 +224,26 @@ def _ptr(a):
     raise TypeError(type(a))
 
 
+_DTYPE_NAMES: dict = {}
+
+
+def _dtype_name(t) -> str:
+    """"bfloat16" for a tensor of torch.bfloat16 and so on, without importing torch."""
+    name = _DTYPE_NAMES.get(t.dtype)
+    if name is None:
+        name = _DTYPE_NAMES[t.dtype] = str(t.dtype).replace("torch.", "")
+    return name
+
+
 def _rows(t, width):
     """(pointer, row stride) of a 2-D device tensor of at least `width` values a row, the
     values of a row next to each other; (None, width) for None."""
     if t is None:
         return None, width
-    if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] < width:
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if cols < width or (step != 1 and cols > 1):
         raise ValueError(f"rows of at least {width} adjacent values expected, got {tuple(t.shape)}")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]))
+    return t.data_ptr(), (ld if rows > 1 else max(ld, cols))
 
 
 def _stream(s):
@@ -525,7 +537,7 @@ def attention_tf32(cfg: MhaConfig, batch, seq, q, q_lo, k, k_lo, v, v_lo, out, o
 
 def rope_table(max_pos, head_dim, table, theta=10000.0, stream=None):
     """(cos, sin) of pos / theta^(2i/head_dim) into table [max_pos, head_dim/2, 2] FP32."""
-    check(lib().welvet_b200_rope_table(max_pos, head_dim, theta, _typed(table, "torch.float32", max_pos * head_dim),
+    check(lib().welvet_b200_rope_table(max_pos, head_dim, theta, _typed(table, "float32", max_pos * head_dim),
                                        _stream(stream)))
 
 
@@ -533,25 +545,27 @@ def _typed(t, dtype, numel=0):
     """Device pointer of a contiguous tensor of the given dtype and at least numel values."""
     if t is None:
         return None
-    if str(t.dtype) != dtype or not t.is_contiguous() or t.numel() < numel:
+    if _dtype_name(t) != dtype or t.numel() < numel or not t.is_contiguous():
         raise ValueError(f"contiguous {dtype} of at least {numel} values expected, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _norm_call(q, k, q_out, k_out, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod):
-    tokens = q.shape[0]
-    for t in (k, q_out, k_out):
+def _norm_call(q, k, others, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod):
+    """(io_bf16, the leading arguments, row widths) of a norm call; `others` have the
+    tokens and the dtype of q."""
+    tokens, qd = q.shape
+    kd = 0 if k is None else k.shape[1]
+    for t in (k, *others):
         if t is not None and (t.shape[0] != tokens or t.dtype != q.dtype):
-            raise ValueError("q, k and their outputs need the same tokens and dtype")
-    io = {"torch.bfloat16": 1, "torch.float32": 0}.get(str(q.dtype))
-    if io is None or q.shape[1] % head_dim or (k is not None and k.shape[1] % head_dim):
+            raise ValueError("q, k, their outputs and gradients need the same tokens and dtype")
+    io = {"bfloat16": 1, "float32": 0}.get(_dtype_name(q))
+    if io is None or qd % head_dim or kd % head_dim:
         raise ValueError("BF16 or FP32 rows of whole heads expected")
-    heads, kv_heads = q.shape[1] // head_dim, 0 if k is None else k.shape[1] // head_dim
-    args = [tokens, heads, kv_heads, head_dim, eps, _typed(q_gamma, "torch.float32", head_dim),
-            _typed(k_gamma, "torch.float32", head_dim), _typed(rope, "torch.float32"),
-            0 if rope is None else rope.numel() // head_dim, _typed(positions, "torch.int32", tokens), pos_mod,
-            *_rows(q, heads * head_dim), *_rows(k, kv_heads * head_dim)]
-    return io, args, (heads * head_dim, kv_heads * head_dim)
+    args = (tokens, qd // head_dim, kd // head_dim, head_dim, eps, _typed(q_gamma, "float32", head_dim),
+            _typed(k_gamma, "float32", head_dim), _typed(rope, "float32"),
+            0 if rope is None else rope.numel() // head_dim, _typed(positions, "int32", tokens), pos_mod,
+            *_rows(q, qd), *_rows(k, kd))
+    return io, args, qd, kd
 
 
 def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1e-6, rope=None, positions=None,
@@ -559,7 +573,7 @@ def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1
     """RMS norm of every query and key head with the rotation in the same pass
     (welvet_b200_qk_norm_rope_forward): rows [tokens, heads * head_dim] (may be views of
     one packed row; k may be None), outputs may be the inputs."""
-    io, args, (qd, kd) = _norm_call(q, k, q_out, k_out, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    io, args, qd, kd = _norm_call(q, k, (q_out, k_out), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
     check(lib().welvet_b200_qk_norm_rope_forward(*args, *_rows(q_out, qd), *_rows(k_out, kd), io, _stream(stream)))
 
 
@@ -573,15 +587,13 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, dq_gamma, dk_gamma, head
     """Gradient of qk_norm_rope (welvet_b200_qk_norm_rope_backward): dq, dk from the
     forward's inputs and the gradients of its outputs, dq_gamma / dk_gamma [head_dim]
     overwritten with the sums over all rows."""
-    io, args, (qd, kd) = _norm_call(q, k, dq, dk, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
-    for t in (dq_out, dk_out):
-        if t is not None and (t.shape[0] != q.shape[0] or t.dtype != q.dtype):
-            raise ValueError("the gradients need the tokens and dtype of q")
+    io, args, qd, kd = _norm_call(q, k, (dq_out, dk_out, dq, dk), head_dim, q_gamma, k_gamma, eps, rope, positions,
+                                  pos_mod)
     if workspace.numel() * workspace.element_size() < qk_norm_rope_workspace(head_dim):
         raise ValueError("workspace smaller than qk_norm_rope_workspace(head_dim)")
     check(lib().welvet_b200_qk_norm_rope_backward(
         *args, *_rows(dq_out, qd), *_rows(dk_out, kd), *_rows(dq, qd), *_rows(dk, kd),
-        _typed(dq_gamma, "torch.float32", head_dim), _typed(dk_gamma, "torch.float32", head_dim), _ptr(workspace), io,
+        _typed(dq_gamma, "float32", head_dim), _typed(dk_gamma, "float32", head_dim), _ptr(workspace), io,
         _stream(stream)))
 
 
@@ -599,13 +611,13 @@ class Kv8Cache:
         batch, max_pages = block_table.shape
         n = pages * kv_heads * (self.PAGE // self.BLOCK)
         self.tensors = (k, v, k_scale, v_scale, block_table, ctx_len)
-        self.args = _Kv8CacheArgs(_ptr(k), _ptr(v), _typed(k_scale, "torch.float32", n),
-                                  _typed(v_scale, "torch.float32", n), _typed(block_table, "torch.int32"),
-                                  _typed(ctx_len, "torch.int32", batch), batch, pages, max_pages, kv_heads, head_dim)
+        self.args = _Kv8CacheArgs(_ptr(k), _ptr(v), _typed(k_scale, "float32", n),
+                                  _typed(v_scale, "float32", n), _typed(block_table, "int32"),
+                                  _typed(ctx_len, "int32", batch), batch, pages, max_pages, kv_heads, head_dim)
 
 
 def _bf16_rows(t, rows, width):
-    if str(t.dtype) != "torch.bfloat16" or t.shape[0] < rows:
+    if _dtype_name(t) != "bfloat16" or t.shape[0] < rows:
         raise ValueError(f"{rows} BF16 rows expected, got {t.dtype} {tuple(t.shape)}")
     return _rows(t, width)
 
@@ -615,9 +627,9 @@ def kv8_append(cache: Kv8Cache, seq, k, v, rope=None, seq_lens=None, stream=None
     views of packed rows) to the cache (welvet_b200_kv8_append)."""
     c = cache.args
     width = c.kv_heads * c.head_dim
-    check(lib().welvet_b200_kv8_append(C.byref(c), seq, _typed(seq_lens, "torch.int32", c.batch),
+    check(lib().welvet_b200_kv8_append(C.byref(c), seq, _typed(seq_lens, "int32", c.batch),
                                        *_bf16_rows(k, c.batch * seq, width), *_bf16_rows(v, c.batch * seq, width),
-                                       _typed(rope, "torch.float32"), 0 if rope is None else rope.numel() // c.head_dim,
+                                       _typed(rope, "float32"), 0 if rope is None else rope.numel() // c.head_dim,
                                        _stream(stream)))
 
 
@@ -626,7 +638,7 @@ def kv8_attention(cfg: MhaConfig, cache: Kv8Cache, seq, q, out, max_ctx, seq_len
     (welvet_b200_kv8_attention)."""
     c = cache.args
     width = (cfg.head_count if cfg.head_count > 0 else cfg.num_heads) * c.head_dim
-    check(lib().welvet_b200_kv8_attention(C.byref(cfg), C.byref(c), seq, _typed(seq_lens, "torch.int32", c.batch),
+    check(lib().welvet_b200_kv8_attention(C.byref(cfg), C.byref(c), seq, _typed(seq_lens, "int32", c.batch),
                                           max_ctx, *_bf16_rows(q, c.batch * seq, width),
                                           *_bf16_rows(out, c.batch * seq, width), _stream(stream)))
 
