@@ -29,8 +29,11 @@
 //
 // Roles: softmax warpgroups (thread = TMEM lane = key; NCG column groups share a tile,
 // NTG tile groups take tiles in turn with an O, ref and l of their own, joined at the
-// end), a TMA warp (pages of codes and their four scales into a ring of 128-key
-// stages), an MMA warp (S_0, S_1, then PV_i, S_{i+2}; S and P double-buffered).
+// end), a TMA warp (pages of codes and their four scales into rings of 128-key tiles),
+// an MMA warp (S_0, S_1, then PV_i with S_{i+2}; S and P double-buffered). Keys and
+// values have rings of their own: a key tile is free as soon as its S is done, two
+// tiles before its values are, so equal rings leave each three tiles of time to load
+// (one ring of both left a load one tile: 1.1 against 0.6 k cycles a tile).
 // A long context is split over a cluster of up to 16 CTAs whose partial (ref, l, O)
 // are joined through distributed shared memory in rank order: no workspace, no second
 // launch, the same bits every time.
@@ -43,6 +46,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 namespace wv {
 namespace {
@@ -55,26 +59,27 @@ constexpr int kMaxCluster = 16;
 
 // Column and tile groups: enough softmax warps to hide the latency of a tile's chain
 // (MMA, TMEM load, exponentials, conversion, store, MMA) within the registers.
-template <int HD, int RT> struct KT {
+template <int HD, int RT, bool DEEP> struct KT {
   static constexpr int NCG = RT == 64 ? 4 : RT == 32 ? 2 : 1;
   static constexpr int NTG = RT == 64 || (RT == 32 && HD == 64) ? 1 : 2;
   static constexpr int CPW = RT / NCG;              // columns of a warpgroup
   static constexpr int SOFT_WARPS = NCG * NTG * 4;
   static constexpr int THREADS = SOFT_WARPS * 32 + 64;
   static constexpr int TILE = kKeys * HD;           // bytes of a K or V tile
-  static constexpr int STAGE = 2 * TILE;
   static constexpr int NS = 2 * RT;                 // columns of S: hi | lo
   static constexpr int NO = RT == 8 ? 32 : 3 * RT;  // columns of O and P: three terms
   static constexpr int O_COL = 2 * NS;              // TMEM: S_0 | S_1 | O of the tile groups
   static constexpr int COLS = O_COL + NTG * NO;
   static constexpr int TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-  static constexpr int STAGES = TMEM < 512 ? (HD == 64 ? 4 : 3) : (HD == 64 ? 8 : 4);
+  static constexpr int STAGES = (DEEP ? 6 : RT == 64 || TMEM == 512 ? 4 : HD == 64 ? 2 : 3) * (HD == 64 ? 2 : 1);  // of K, and of V
+  static constexpr int SCALES = STAGES + 2;  // scales outlive their key tile by two tiles
+  static constexpr int OFF_V = STAGES * TILE;
   static constexpr int P_BYTES = kKeys * NO;
   static constexpr int Q_BYTES = NS * HD;
-  static constexpr int OFF_P = STAGES * STAGE;
+  static constexpr int OFF_P = 2 * STAGES * TILE;
   static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
-  static constexpr int OFF_SC = OFF_Q + Q_BYTES;          // scales: [stage][K, V][8]
-  static constexpr int OFF_OUT = OFF_SC + STAGES * 64;    // output element of a column (64 bits), -1: none
+  static constexpr int OFF_SC = OFF_Q + Q_BYTES;          // scales: [slot][K, V][8]
+  static constexpr int OFF_OUT = OFF_SC + SCALES * 64;    // output element of a column (64 bits), -1: none
   static constexpr int OFF_QF = OFF_OUT + RT * 8;         // factor of a column's scores
   static constexpr int OFF_REF = OFF_QF + RT * 4;         // [NTG][RT] bias - reference
   static constexpr int OFF_FAC = OFF_REF + NTG * RT * 4;  // [NTG][RT] rescaling factors
@@ -83,7 +88,7 @@ template <int HD, int RT> struct KT {
   static constexpr int OFF_SLOPE = OFF_QHI + RT * 4;
   static constexpr int OFF_RED = OFF_SLOPE + RT * 4;      // [NTG][4 warps][RT]
   static constexpr int OFF_BAR = OFF_RED + NTG * 4 * RT * 4;
-  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (2 * STAGES + 7) + 32;
+  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (4 * STAGES + SCALES + 7) + 32;
   // resident CTAs of an SM
   static constexpr int BY_SMEM = 228 * 1024 / (SMEM + 1024), BY_TMEM = 512 / TMEM;
   static constexpr int PER_SM = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
@@ -93,7 +98,7 @@ template <int HD, int RT> struct KT {
   static_assert(SMEM > 72 * 1024 && (TMEM < 512 || SMEM > (228 - 72) * 1024), "TMEM columns of co-resident CTAs");
   // Partial O, [RT][HD] FP32, over the stages, and the cluster's [16][RT] references,
   // sums and weights over P, once every MMA has read them.
-  static_assert(RT * HD * 4 <= STAGES * STAGE && 3 * 16 * RT * 4 <= 2 * P_BYTES, "joining areas");
+  static_assert(RT * HD * 4 <= 2 * STAGES * TILE && 3 * 16 * RT * 4 <= 2 * P_BYTES, "joining areas");
   static_assert(COLS <= TMEM, "TMEM columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -210,17 +215,20 @@ WV_DEV float ld_peer(uint32_t addr) {
   return v;
 }
 
-template <int HD, int RT, bool ALIBI>
-__global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
+template <int HD, int RT, bool DEEP, bool ALIBI>
+__global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::PER_SM)
     kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const Kv8AttnArgs a, int splits) {
-  using T = KT<HD, RT>;
+  using T = KT<HD, RT, DEEP>;
   constexpr int CPW = T::CPW, ST = T::STAGES, NTG = T::NTG, NCG = T::NCG, kSoftWarps = T::SOFT_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::OFF_BAR);
-  uint64_t* empty = full + ST;
-  uint64_t* s_full = empty + ST;  // [2]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + T::OFF_BAR);
+  uint64_t* k_empty = k_full + ST;
+  uint64_t* v_full = k_empty + ST;
+  uint64_t* v_empty = v_full + ST;
+  uint64_t* sc_full = v_empty + ST;  // [SCALES] a tile's scales
+  uint64_t* s_full = sc_full + T::SCALES;  // [2]
   uint64_t* p_full = s_full + 2;  // [2]
   uint64_t* pv_done = p_full + 2; // [2]
   uint64_t* q_full = pv_done + 2;
@@ -236,10 +244,7 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   const int warp = (int)warp_id(), lane = (int)lane_id();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
+    for (int s = 0; s < 4 * ST + T::SCALES; ++s) mbar_init(&k_full[s], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], NCG * 4);  // the warps that share a tile
@@ -289,9 +294,12 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     const int* bt = a.c.block_table + (size_t)b * a.c.max_pages;
     const int p0 = base0 / kKv8Page;
     const int np = tiles > 0 ? min((k1 + kKv8Page - 1) / kKv8Page - p0, 2 * tiles) : 0;  // pages of this CTA
-    int next = lane < np ? bt[p0 + lane] : 0, ids = 0;
-    for (int j = 0; j < tiles; ++j) {
-      if (j % 16 == 0) {  // 32 page ids at a time, requested one batch ahead
+    // Page ids 32 at a time, requested one batch ahead; V follows two tiles behind K,
+    // as PV_j follows S_{j+2}.
+    int next = lane < np ? bt[p0 + lane] : 0, ids = 0, held = 0;
+    for (int j = 0; j < tiles + 2; ++j) {
+      if (j % 16 == 0) {
+        held = ids;
         ids = next;
         const int at = 2 * j + 32 + lane;
         next = at < np ? bt[p0 + at] : 0;
@@ -300,27 +308,45 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
           ids = 0;
         }
       }
-      const int s = j % ST;
-      if (ok && lane == 0 && j >= ST) ok = mbar_wait(&empty[s], ((j / ST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      if (!ok) {  // the copies in flight land before the CTA ends (bounded)
-        int none = 0;
-        for (int k = max(0, j - ST); lane == 0 && k < j; ++k)
-          mbar_wait_for(&full[k % ST], (k / ST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
-        break;
-      }
-      const int two = 2 * j + 1 < np ? 2 : 1;
-      const int id[2] = {__shfl_sync(0xffffffffu, ids, (2 * j) & 31), __shfl_sync(0xffffffffu, ids, (2 * j + 1) & 31)};
-      if (lane == 0) {
-        uint8_t* kt = smem + s * T::STAGE;
-        float* sc = reinterpret_cast<float*>(smem + T::OFF_SC + s * 64);
-        mbar_arrive_expect_tx(&full[s], two * (2 * kKv8Page * HD + 32));
-        for (int i = 0; i < two; ++i) {
-          const int ph = id[i] * a.c.kv_heads + kh;
-          bulk_load(sc + i * 4, a.c.k_scale + (size_t)ph * kKv8Subs, 16, &full[s]);
-          bulk_load(sc + 8 + i * 4, a.c.v_scale + (size_t)ph * kKv8Subs, 16, &full[s]);
-          tma_load_2d(kt + i * kKv8Page * HD, &tmK, &full[s], 0, ph * kKv8Page);
-          tma_load_2d(kt + T::TILE + i * kKv8Page * HD, &tmV, &full[s], 0, ph * kKv8Page);
+      // K_j and the scales of tile j, then V_{j-2}
+      const int kp[2] = {__shfl_sync(0xffffffffu, ids, (2 * j) & 31), __shfl_sync(0xffffffffu, ids, (2 * j + 1) & 31)};
+      const int jv = j - 2, from = j % 16 < 2 ? held : ids;
+      const int vp[2] = {__shfl_sync(0xffffffffu, from, (2 * jv) & 31), __shfl_sync(0xffffffffu, from, (2 * jv + 1) & 31)};
+      if (lane == 0 && ok) {
+        if (j < tiles) {
+          const int s = j % ST, two = 2 * j + 1 < np ? 2 : 1;
+          if (j >= ST) ok = mbar_wait(&k_empty[s], ((j / ST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
+          if (ok) {
+            float* sc = reinterpret_cast<float*>(smem + T::OFF_SC + (j % T::SCALES) * 64);
+            uint64_t* sb = &sc_full[j % T::SCALES];
+            mbar_arrive_expect_tx(&k_full[s], two * kKv8Page * HD);
+            mbar_arrive_expect_tx(sb, two * 32);
+            for (int i = 0; i < two; ++i) {
+              const int ph = kp[i] * a.c.kv_heads + kh;
+              tma_load_2d(smem + s * T::TILE + i * kKv8Page * HD, &tmK, &k_full[s], 0, ph * kKv8Page);
+              bulk_load(sc + i * 4, a.c.k_scale + (size_t)ph * kKv8Subs, 16, sb);
+              bulk_load(sc + 8 + i * 4, a.c.v_scale + (size_t)ph * kKv8Subs, 16, sb);
+            }
+          }
+        }
+        if (jv >= 0 && ok) {
+          const int s = jv % ST, two = 2 * jv + 1 < np ? 2 : 1;
+          if (jv >= ST) ok = mbar_wait(&v_empty[s], ((jv / ST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
+          if (ok) {
+            mbar_arrive_expect_tx(&v_full[s], two * kKv8Page * HD);
+            for (int i = 0; i < two; ++i)
+              tma_load_2d(smem + T::OFF_V + s * T::TILE + i * kKv8Page * HD, &tmV, &v_full[s], 0,
+                          (vp[i] * a.c.kv_heads + kh) * kKv8Page);
+          }
+        }
+        if (!ok) {  // the copies in flight land before the CTA ends (bounded)
+          int none = 0;
+          for (int k = max(0, j - ST); k < min(j, tiles); ++k) {
+            mbar_wait_for(&k_full[k % ST], (k / ST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
+            mbar_wait_for(&sc_full[k % T::SCALES], (k / T::SCALES) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
+          }
+          for (int k = max(0, jv - ST); k < jv; ++k)
+            mbar_wait_for(&v_full[k % ST], (k / ST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
         }
       }
     }
@@ -339,59 +365,95 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.err, code)) != 0;
     };
-    auto issue_s = [&](int j) -> bool {
-      const int s = j % ST;
-      if (!wait(&full[s], (j / ST) & 1, kErrWaitFull)) return false;
-      tc_fence_after();
-      const uint32_t k_lo = sdesc_lo(base + s * T::STAGE, 16);
-      if (lead) {
-#pragma unroll
-        for (int kk = 0; kk < HD / 32; ++kk)
-          umma_f8(tmem + (uint32_t)((j & 1) * T::NS), k_lo + kk * 2, HI_KV, q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
-        umma_commit(&s_full[j & 1]);
-      }
-      __syncwarp();
-      return true;
+    // S_j: HD / 32 MMAs; PV_i: kKeys / 32. An MMA waits for the one before it on the
+    // same accumulator, so PV_i and S_{i+2} are issued in turn when both can run.
+    const auto s_mma = [&](int j, int kk) {
+      umma_f8(tmem + (uint32_t)((j & 1) * T::NS), sdesc_lo(base + (j % ST) * T::TILE, 16) + kk * 2, HI_KV,
+              q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
     };
+    const auto pv_mma = [&](int i, int kk) {
+      umma_f8(tmem + T::O_COL + (i % NTG) * T::NO, sdesc_lo(base + T::OFF_V + (i % ST) * T::TILE, 16) + kk * (32 * HD / 16),
+              HI_KV, sdesc_lo(base + T::OFF_P + (i & 1) * T::P_BYTES, 128) + kk * 32, HI_P, IDESC_PV,
+              kk > 0 || i >= NTG ? 1u : 0u);
+    };
+    constexpr int kS = HD / 32, kPV = kKeys / 32;
     if (tiles > 0) ok = wait(q_full, 0, kErrWaitOther);
-    for (int j = 0; ok && j < min(2, tiles); ++j) ok = issue_s(j);
-    for (int i = 0; ok && i < tiles; ++i) {
-      ok = wait(&p_full[i & 1], (i >> 1) & 1, kErrWaitOther);
+    for (int j = 0; ok && j < min(2, tiles); ++j) {
+      ok = wait(&k_full[j % ST], (j / ST) & 1, kErrWaitFull);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t v_lo = sdesc_lo(base + (i % ST) * T::STAGE + T::TILE, 16);
-      const uint32_t p_lo = sdesc_lo(base + T::OFF_P + (i & 1) * T::P_BYTES, 128);
-      const uint32_t first = i >= NTG ? 1u : 0u;
       if (lead) {
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 32; ++kk)
-          umma_f8(tmem + T::O_COL + (i % NTG) * T::NO, v_lo + kk * (32 * HD / 16), HI_KV, p_lo + kk * 32, HI_P, IDESC_PV,
-                  kk > 0 ? 1u : first);
-        umma_commit(&empty[i % ST]);
-        umma_commit(&pv_done[i & 1]);
+        for (int kk = 0; kk < kS; ++kk) s_mma(j, kk);
+        umma_commit(&s_full[j & 1]);
+        umma_commit(&k_empty[j % ST]);
       }
       __syncwarp();
-      if (i + 2 < tiles) ok = issue_s(i + 2);
+    }
+    for (int i = 0; ok && i < tiles; ++i) {
+      ok = wait(&v_full[i % ST], (i / ST) & 1, kErrWaitFull) && wait(&p_full[i & 1], (i >> 1) & 1, kErrWaitOther);
+      if (!ok) break;
+      const int j = i + 2;
+      uint64_t* jf = &k_full[j % ST];
+      const uint32_t jp = (j / ST) & 1;
+      const bool both = j < tiles && __all_sync(0xffffffffu, mbar_test_wait(jf, jp));
+      tc_fence_after();
+      if (lead) {
+#pragma unroll
+        for (int kk = 0; kk < kPV; ++kk) {
+          pv_mma(i, kk);
+          if (both && kk < kS) s_mma(j, kk);
+        }
+        if (both) {
+          umma_commit(&s_full[j & 1]);
+          umma_commit(&k_empty[j % ST]);
+        }
+        umma_commit(&pv_done[i & 1]);
+        umma_commit(&v_empty[i % ST]);
+      }
+      __syncwarp();
+      if (j < tiles && !both) {
+        ok = wait(jf, jp, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+        if (lead) {
+#pragma unroll
+          for (int kk = 0; kk < kS; ++kk) s_mma(j, kk);
+          umma_commit(&s_full[j & 1]);
+          umma_commit(&k_empty[j % ST]);
+        }
+        __syncwarp();
+      }
     }
   } else {
     // ---- queries: hi and lo codes, [16-byte chunk of hd][RT hi rows, RT lo rows][16]
-    for (int c = warp; c < RT; c += kSoftWarps) {
-      const int t = (r0 + c) / G, h = kh * G + (r0 + c) - t * G;
-      const bool live = t >= t0 && t <= t1;
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + t) * a.ldq + (size_t)h * HD;
-      float x[HD / 32], m = 0.f;
+    constexpr int NQ = (RT + kSoftWarps - 1) / kSoftWarps;  // columns of a warp, all loads first
+    float x[NQ][HD / 32];
+    int tq[NQ], hq[NQ];
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        x[i] = live ? __bfloat162float(q[lane + 32 * i]) : 0.f;
-        m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
-      }
+    for (int k = 0; k < NQ; ++k) {
+      const int c = warp + k * kSoftWarps, t = (r0 + c) / G, h = kh * G + (r0 + c) - t * G;
+      tq[k] = t;
+      hq[k] = h;
+      const bool live = c < RT && t >= t0 && t <= t1;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + t) * a.ldq + (size_t)h * HD;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) x[k][i] = live ? __bfloat162float(q[lane + 32 * i]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) {
+      const int c = warp + k * kSoftWarps;
+      if (c >= RT) break;
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) m = fmaxf(m, x[k][i] - x[k][i] == 0.f ? fabsf(x[k][i]) : INFINITY);
       m = warp_max(m);
       const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
-      const float s = bad ? 1.f : kv8_scale(m);
+      const float s = bad ? 1.f : kv8_scale(m), rs = 1.f / s;  // powers of two
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
         const int e = lane + 32 * i;
-        const float y = bad ? 0.f : x[i] / s;
+        const float y = bad ? 0.f : x[k][i] * rs;
         const uint32_t hi = e4m3x2(y, 0.f);
         const uint32_t lo = e4m3x2(y - e4m3x2_value(hi).x, 0.f);
         uint8_t* dst = smem + T::OFF_Q + (e / 16) * (T::NS * 16) + e % 16;
@@ -399,6 +461,8 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
         dst[(RT + c) * 16] = (uint8_t)lo;
       }
       if (lane == 0) {
+        const int t = tq[k], h = hq[k];
+        const bool live = t >= t0 && t <= t1;
         qf[c] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
         for (int g = 0; g < NTG; ++g) refs[g * RT + c] = kNoRef;
         // a column without a query sees whatever there is; its output is zero, or none
@@ -424,18 +488,19 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
 #pragma unroll
     for (int c = 0; c < CPW / 2; ++c) l2[c] = 0ull;
     for (int i = tg; i < tiles; i += NTG) {
-      const int s = i % ST, base = base0 + i * kKeys, kpos = base + key;
+      const int base = base0 + i * kKeys, kpos = base + key;
       // After a wait that gave up, the tiles are still walked (the waits return at once):
       // the warpgroup's barriers need every thread.
-      ok = mbar_wait(&full[s], (i / ST) & 1, abort_flag, a.err, kErrWaitFull) && ok;  // the scales
-      const float* sc = reinterpret_cast<const float*>(smem + T::OFF_SC + s * 64);
+      ok = mbar_wait(&sc_full[i % T::SCALES], (i / T::SCALES) & 1, abort_flag, a.err, kErrWaitFull) && ok;
+      const float* sc = reinterpret_cast<const float*>(smem + T::OFF_SC + (i % T::SCALES) * 64);
       const bool on = kpos < k1;
       const float ks = sc[key >> 4], vs = sc[8 + (key >> 4)];
       float ev;
       asm("lg2.approx.f32 %0, %1;" : "=f"(ev) : "f"(vs));
       const float inv = on && vs == vs ? __fdividef(1.f, vs) : 0.f;
       if (!on && c0 == 0) {  // rows past the context may hold NaN codes: 0 * NaN
-        uint8_t* row = smem + s * T::STAGE + T::TILE + key * HD;
+        ok = mbar_wait(&v_full[i % ST], (i / ST) & 1, abort_flag, a.err, kErrWaitFull) && ok;
+        uint8_t* row = smem + T::OFF_V + (i % ST) * T::TILE + key * HD;
 #pragma unroll 1
         for (int x = 0; x < HD; x += 16) *reinterpret_cast<uint4*>(row + x) = make_uint4(0u, 0u, 0u, 0u);
       }
@@ -668,8 +733,9 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   cluster_sync();  // no CTA leaves while another reads its partials
 }
 
-template <int HD, int RT> cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
-  using T = KT<HD, RT>;
+template <int HD, int RT, bool DEEP>
+cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
+  using T = KT<HD, RT, DEEP>;
   const int group = a.heads / a.c.kv_heads;
   const int64_t row_tiles = ((int64_t)a.seq * group + RT - 1) / RT;
   const int64_t pairs = row_tiles * a.c.kv_heads * a.batch;
@@ -678,7 +744,8 @@ template <int HD, int RT> cudaError_t launch(const CUtensorMap& mk, const CUtens
   const int keys = a.window > 0 ? std::min(a.max_ctx, a.window + a.seq + kKv8Page) : a.max_ctx;
   int splits = 1;
   while (splits < kMaxCluster && pairs * splits * 2 <= (int64_t)a.sm_count * T::PER_SM && splits * 2 * kKeys <= keys) splits *= 2;
-  auto kern = a.alibi ? kv8_attn_kernel<HD, RT, true> : kv8_attn_kernel<HD, RT, false>;
+  if (getenv("WVT_S")) splits = atoi(getenv("WVT_S"));
+  auto kern = a.alibi ? kv8_attn_kernel<HD, RT, DEEP, true> : kv8_attn_kernel<HD, RT, DEEP, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
   if (e == cudaSuccess && splits > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
@@ -701,10 +768,11 @@ template <int HD, int RT> cudaError_t launch(const CUtensorMap& mk, const CUtens
 
 template <int HD> cudaError_t launch_hd(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.seq * (a.heads / a.c.kv_heads);
-  if (rows <= 8) return launch<HD, 8>(mk, mv, a, s);
-  if (rows <= 16) return launch<HD, 16>(mk, mv, a, s);
-  if (rows <= 32) return launch<HD, 32>(mk, mv, a, s);
-  return launch<HD, 64>(mk, mv, a, s);
+  const bool deep = getenv("WVT_D") && atoi(getenv("WVT_D"));
+  if (rows <= 8) return deep ? launch<HD, 8, true>(mk, mv, a, s) : launch<HD, 8, false>(mk, mv, a, s);
+  if (rows <= 16) return deep ? launch<HD, 16, true>(mk, mv, a, s) : launch<HD, 16, false>(mk, mv, a, s);
+  if (rows <= 32) return launch<HD, 32, false>(mk, mv, a, s);
+  return launch<HD, 64, false>(mk, mv, a, s);
 }
 
 }  // namespace
