@@ -12,10 +12,10 @@
 // What the small operands lose in 8 bits is kept in more of them:
 //   * a query row, scaled by a power of two to at most 448, is a sum of two E4M3 codes:
 //     exact to 2^-10 of 448, i.e. BF16 queries to 2^-19 of the row's largest value;
-//   * a probability, rounded to FP16, is a sum of three E5M2 codes (3 significant bits
-//     each, rounded to nearest in turn): a relative 2^-9, down to 2^-28 of the largest
-//     before the codes run out, so that long tails of small probabilities still add
-//     up. E4M3 codes would be finer but end at 2^-20 of the largest.
+//   * a probability, rounded to FP16, is hi + lo/8 + lo2/64 in E5M2 codes (3 significant
+//     bits each, rounded to nearest in turn): a relative 2^-9 down to 2^-19 of the
+//     largest, and 2^-28 of the largest below that, so that long tails of small
+//     probabilities still add up. E4M3 codes would be finer but end at 2^-14.
 // The codes of one sum are columns side by side (2 RT of S, 3 RT of O), added when
 // read: a 128-row MMA of 32 bytes takes about 60 cycles for any N up to 128, so one
 // wide MMA is cheaper than several narrow ones into the same columns.
@@ -23,9 +23,9 @@
 //
 // Softmax in the log2 domain with the value scale folded in: z = s kscale qscale
 // scale log2e + log2(vscale), p = 2^(z - ref), O += p * code, l += p / vscale. ref is a
-// column's running maximum of z, raised only when some z exceeds it by more than 2^4
-// (E5M2 has the room), so that most tiles need one vote and no maximum at all; when
-// it moves, O and l are rescaled.
+// column's running maximum of z, raised only when some p would exceed 2^10 (E5M2 has the
+// room), so that after the first tile one vote and no maximum is the rule; when it
+// moves, O and l are rescaled.
 //
 // Roles: softmax warpgroups (thread = TMEM lane = key; NCG column groups share a tile,
 // NTG tile groups take tiles in turn with an O, ref and l of their own, joined at the
@@ -45,23 +45,24 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
-#include <cstdlib>
+#include <type_traits>
 
 namespace wv {
 namespace {
 
 constexpr int kKeys = 128;          // keys of a tile: two pages
-constexpr float kBias = 11.f;       // log2 of p at the reference
-constexpr float kSlack = 4.f;       // z may exceed the reference by this much (p <= 2^15)
-constexpr float kNoRef = 1e30f;     // bias - ref of a column that has seen no key
+constexpr float kBias = 5.f;        // log2 of p at the reference
+constexpr float kSlack = 10.f;      // z may exceed the reference by this much (p <= 2^15)
+constexpr float kNoRef = 1e30f;     // bias - ref of a column that has seen no key, when joining
 constexpr int kMaxCluster = 16;
 
 // Column and tile groups: enough softmax warps to hide the latency of a tile's chain
 // (MMA, TMEM load, exponentials, conversion, store, MMA) within the registers.
-template <int HD, int RT, bool DEEP> struct KT {
+template <int HD, int RT> struct KT {
   static constexpr int NCG = RT == 64 ? 4 : RT == 32 ? 2 : 1;
-  static constexpr int NTG = RT == 64 || (RT == 32 && HD == 64) ? 1 : 2;
+  static constexpr int NTG = HD == 128 && (RT == 8 || RT == 32) ? 2 : 1;
   static constexpr int CPW = RT / NCG;              // columns of a warpgroup
   static constexpr int SOFT_WARPS = NCG * NTG * 4;
   static constexpr int THREADS = SOFT_WARPS * 32 + 64;
@@ -71,34 +72,39 @@ template <int HD, int RT, bool DEEP> struct KT {
   static constexpr int O_COL = 2 * NS;              // TMEM: S_0 | S_1 | O of the tile groups
   static constexpr int COLS = O_COL + NTG * NO;
   static constexpr int TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-  static constexpr int STAGES = (DEEP ? 6 : RT == 64 || TMEM == 512 ? 4 : HD == 64 ? 2 : 3) * (HD == 64 ? 2 : 1);  // of K, and of V
-  static constexpr int SCALES = STAGES + 2;  // scales outlive their key tile by two tiles
-  static constexpr int OFF_V = STAGES * TILE;
+  // tiles of the K and of the V ring
+  static constexpr int KST = HD == 128 ? (RT == 32 ? 5 : 3) : (RT == 64 ? 7 : RT == 8 ? 3 : 4);
+  static constexpr int VST = (HD == 64 && RT == 8) || (HD == 128 && RT == 16) ? KST - 1 : KST;
+  static constexpr int SCALES = KST + 2;  // scales outlive their key tile by two tiles
   static constexpr int P_BYTES = kKeys * NO;
   static constexpr int Q_BYTES = NS * HD;
-  static constexpr int OFF_P = 2 * STAGES * TILE;
+  static constexpr int OFF_V = KST * TILE;
+  static constexpr int OFF_P = OFF_V + VST * TILE;
   static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
-  static constexpr int OFF_SC = OFF_Q + Q_BYTES;          // scales: [slot][K, V][8]
+  static constexpr int OFF_IN = OFF_Q + Q_BYTES;          // joining: [split][RT HD / splits] partial O
+  static constexpr int OFF_INL = OFF_IN + RT * HD * 4;    // ... and (reference, sum) of their columns
+  static constexpr int OFF_SC = OFF_INL + 8 * (RT > 16 ? RT : 16);  // scales: [slot][K, V][8]
   static constexpr int OFF_OUT = OFF_SC + SCALES * 64;    // output element of a column (64 bits), -1: none
   static constexpr int OFF_QF = OFF_OUT + RT * 8;         // factor of a column's scores
   static constexpr int OFF_REF = OFF_QF + RT * 4;         // [NTG][RT] bias - reference
   static constexpr int OFF_FAC = OFF_REF + NTG * RT * 4;  // [NTG][RT] rescaling factors
-  static constexpr int OFF_L = OFF_FAC + NTG * RT * 4;    // [NTG][RT] sums
+  static constexpr int OFF_HAVE = OFF_FAC + NTG * RT * 4; // [NTG][RT] whether a column has seen a key
+  static constexpr int OFF_L = OFF_HAVE + NTG * RT * 4;   // [NTG][RT] sums
   static constexpr int OFF_QHI = OFF_L + NTG * RT * 4;    // last key of a column
   static constexpr int OFF_SLOPE = OFF_QHI + RT * 4;
   static constexpr int OFF_RED = OFF_SLOPE + RT * 4;      // [NTG][4 warps][RT]
   static constexpr int OFF_BAR = OFF_RED + NTG * 4 * RT * 4;
-  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (4 * STAGES + SCALES + 7) + 32;
+  static constexpr int SMEM = 1024 + OFF_BAR + 8 * (2 * (KST + VST) + SCALES + 7) + 32;
   // resident CTAs of an SM
   static constexpr int BY_SMEM = 228 * 1024 / (SMEM + 1024), BY_TMEM = 512 / TMEM;
   static constexpr int PER_SM = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
   // A CTA that waits for TMEM columns while its cluster waits for it could wait for a
-  // CTA of another stream in the same state. Shared memory rules that out: the CTAs of
-  // these kernels that fit an SM together never need more than its 512 columns.
-  static_assert(SMEM > 72 * 1024 && (TMEM < 512 || SMEM > (228 - 72) * 1024), "TMEM columns of co-resident CTAs");
-  // Partial O, [RT][HD] FP32, over the stages, and the cluster's [16][RT] references,
-  // sums and weights over P, once every MMA has read them.
-  static_assert(RT * HD * 4 <= 2 * STAGES * TILE && 3 * 16 * RT * 4 <= 2 * P_BYTES, "joining areas");
+  // CTA of another stream in the same state. Shared memory rules that out: CTAs of these
+  // kernels that fit an SM together never need more than its 512 columns (128 columns
+  // take at least 1/4 of it, 256 columns 1/2 with what is left over too small for a
+  // third CTA, 512 all but what is too small for one).
+  static_assert(SMEM > 50 * 1024 && (TMEM < 256 || SMEM > 91 * 1024) && (TMEM < 512 || SMEM > 178 * 1024) &&
+                    (TMEM < 256 || PER_SM <= 2), "TMEM columns of co-resident CTAs");
   static_assert(COLS <= TMEM, "TMEM columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -149,6 +155,22 @@ template <int N> WV_DEV void tmem_st(uint32_t addr, const uint32_t* r) {
     tmem_st32(addr, *reinterpret_cast<const uint32_t(*)[32]>(r));
   }
 }
+// Shared-memory loads and stores by 32-bit address (a generic access costs an address
+// in 64 bits and a longer path).
+WV_DEV float lds(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+WV_DEV float4 lds4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+WV_DEV void sts(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+WV_DEV void sts4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 // Maximum over the warp; NaN lanes are left out.
 WV_DEV float warp_max(float v) {
   float r;
@@ -182,15 +204,24 @@ template <int N> WV_DEV void wg_sync(int w) {
   else bar_sync<4>();
 }
 template <int WARPS> WV_DEV void soft_sync() { asm volatile("barrier.cta.sync 5, %0;" ::"n"(WARPS * 32) : "memory"); }
-// FP16 pairs to E5M2 codes (nearest), and the FP16 values of two codes: an E5M2 code is
-// the upper byte of the FP16 pattern of its value.
-WV_DEV uint32_t e5m2x2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&v)));
+// Two FP16 pairs to four E5M2 codes (nearest), and the FP16 values of codes 0, 1 and 2,
+// 3 of a word: an E5M2 code is the upper byte of the FP16 pattern of its value.
+WV_DEV uint32_t e5m2x4(__half2 u, __half2 w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 t, v;\n\t"
+      "cvt.rn.satfinite.e5m2x2.f16x2 t, %1;\n\t"
+      "cvt.rn.satfinite.e5m2x2.f16x2 v, %2;\n\t"
+      "mov.b32 %0, {t, v};\n\t}"
+      : "=r"(r)
+      : "r"(*reinterpret_cast<uint32_t*>(&u)), "r"(*reinterpret_cast<uint32_t*>(&w)));
   return r;
 }
-WV_DEV __half2 e5m2x2_value(uint32_t c) {
+WV_DEV __half2 e5m2_lo(uint32_t c) {
   const uint32_t h = __byte_perm(c, 0u, 0x1404);
+  return *reinterpret_cast<const __half2*>(&h);
+}
+WV_DEV __half2 e5m2_hi(uint32_t c) {
+  const uint32_t h = __byte_perm(c, 0u, 0x3424);
   return *reinterpret_cast<const __half2*>(&h);
 }
 WV_DEV uint64_t fmul2(uint64_t a, uint64_t b) {
@@ -209,25 +240,27 @@ WV_DEV uint32_t peer_addr(const void* local, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
   return r;
 }
-WV_DEV float ld_peer(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+WV_DEV void st_peer(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+WV_DEV void st_peer2(uint32_t addr, float v, float w) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v), "f"(w) : "memory");
 }
+// The two halves of cluster_sync.
+WV_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+WV_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-template <int HD, int RT, bool DEEP, bool ALIBI>
-__global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::PER_SM)
+template <int HD, int RT, bool ALIBI>
+__global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     kv8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const Kv8AttnArgs a, int splits) {
-  using T = KT<HD, RT, DEEP>;
-  constexpr int CPW = T::CPW, ST = T::STAGES, NTG = T::NTG, NCG = T::NCG, kSoftWarps = T::SOFT_WARPS;
+  using T = KT<HD, RT>;
+  constexpr int CPW = T::CPW, KST = T::KST, VST = T::VST, NTG = T::NTG, NCG = T::NCG, kSoftWarps = T::SOFT_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + T::OFF_BAR);
-  uint64_t* k_empty = k_full + ST;
-  uint64_t* v_full = k_empty + ST;
-  uint64_t* v_empty = v_full + ST;
-  uint64_t* sc_full = v_empty + ST;  // [SCALES] a tile's scales
+  uint64_t* k_empty = k_full + KST;
+  uint64_t* v_full = k_empty + KST;
+  uint64_t* v_empty = v_full + VST;
+  uint64_t* sc_full = v_empty + VST;  // [SCALES] a tile's scales
   uint64_t* s_full = sc_full + T::SCALES;  // [2]
   uint64_t* p_full = s_full + 2;  // [2]
   uint64_t* pv_done = p_full + 2; // [2]
@@ -238,13 +271,14 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
   float* qf = reinterpret_cast<float*>(smem + T::OFF_QF);
   float* refs = reinterpret_cast<float*>(smem + T::OFF_REF);
   float* facs = reinterpret_cast<float*>(smem + T::OFF_FAC);
+  float* haves = reinterpret_cast<float*>(smem + T::OFF_HAVE);
   float* lsum = reinterpret_cast<float*>(smem + T::OFF_L);
   int* qhi = reinterpret_cast<int*>(smem + T::OFF_QHI);
   float* slope = reinterpret_cast<float*>(smem + T::OFF_SLOPE);
   const int warp = (int)warp_id(), lane = (int)lane_id();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 4 * ST + T::SCALES; ++s) mbar_init(&k_full[s], 1);
+    for (int s = 0; s < 2 * (KST + VST) + T::SCALES; ++s) mbar_init(&k_full[s], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], NCG * 4);  // the warps that share a tile
@@ -264,11 +298,28 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
   const uint32_t tmem = *tmem_holder;
   pdl_wait();  // the append (or whatever filled the cache, q and the lengths) is complete
   pdl_trigger();  // behind the TMEM allocation: a dependent's CTA must not take the columns first
+  if (splits > 1) cluster_arrive();  // waited for before the first access to another CTA
 
-  // ---- this CTA's columns and keys
+  // ---- this CTA's columns and keys; its query rows are requested with the lengths
   const int split = blockIdx.x % splits, b = blockIdx.z;
   const int kh = blockIdx.y, r0 = (int)(blockIdx.x / splits) * RT;
   const int G = a.heads / a.c.kv_heads;
+  constexpr int NQ = (RT + kSoftWarps - 1) / kSoftWarps;  // columns of a softmax warp
+  __nv_bfloat16 xq[NQ][HD / 32];
+  int tq[NQ], hq[NQ];
+  if (warp < kSoftWarps) {
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) {
+      const int c = warp + k * kSoftWarps;
+      tq[k] = (r0 + c) / G;
+      hq[k] = kh * G + (r0 + c) - tq[k] * G;
+      const __nv_bfloat16* q =
+          static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + tq[k]) * a.ldq + (size_t)hq[k] * HD;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+        xq[k][i] = c < RT && tq[k] < a.seq ? q[lane + 32 * i] : __nv_bfloat16(0.f);
+    }
+  }
   const int n = kv8_new(a.seq_lens, b, a.seq);
   const int shift = a.c.ctx_len[b] - n;  // position of the first new token
   const int t0 = max(r0 / G, max(0, -shift)), t1 = min((r0 + RT - 1) / G, n - 1);  // live tokens
@@ -314,8 +365,8 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
       const int vp[2] = {__shfl_sync(0xffffffffu, from, (2 * jv) & 31), __shfl_sync(0xffffffffu, from, (2 * jv + 1) & 31)};
       if (lane == 0 && ok) {
         if (j < tiles) {
-          const int s = j % ST, two = 2 * j + 1 < np ? 2 : 1;
-          if (j >= ST) ok = mbar_wait(&k_empty[s], ((j / ST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
+          const int s = j % KST, two = 2 * j + 1 < np ? 2 : 1;
+          if (j >= KST) ok = mbar_wait(&k_empty[s], ((j / KST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
           if (ok) {
             float* sc = reinterpret_cast<float*>(smem + T::OFF_SC + (j % T::SCALES) * 64);
             uint64_t* sb = &sc_full[j % T::SCALES];
@@ -330,8 +381,8 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
           }
         }
         if (jv >= 0 && ok) {
-          const int s = jv % ST, two = 2 * jv + 1 < np ? 2 : 1;
-          if (jv >= ST) ok = mbar_wait(&v_empty[s], ((jv / ST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
+          const int s = jv % VST, two = 2 * jv + 1 < np ? 2 : 1;
+          if (jv >= VST) ok = mbar_wait(&v_empty[s], ((jv / VST) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty);
           if (ok) {
             mbar_arrive_expect_tx(&v_full[s], two * kKv8Page * HD);
             for (int i = 0; i < two; ++i)
@@ -341,12 +392,12 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
         }
         if (!ok) {  // the copies in flight land before the CTA ends (bounded)
           int none = 0;
-          for (int k = max(0, j - ST); k < min(j, tiles); ++k) {
-            mbar_wait_for(&k_full[k % ST], (k / ST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
+          for (int k = max(0, j - KST); k < min(j, tiles); ++k) {
+            mbar_wait_for(&k_full[k % KST], (k / KST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
             mbar_wait_for(&sc_full[k % T::SCALES], (k / T::SCALES) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
           }
-          for (int k = max(0, jv - ST); k < jv; ++k)
-            mbar_wait_for(&v_full[k % ST], (k / ST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
+          for (int k = max(0, jv - VST); k < jv; ++k)
+            mbar_wait_for(&v_full[k % VST], (k / VST) & 1, &none, a.err, kErrWaitFull, 1000000000ull);
         }
       }
     }
@@ -368,34 +419,34 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
     // S_j: HD / 32 MMAs; PV_i: kKeys / 32. An MMA waits for the one before it on the
     // same accumulator, so PV_i and S_{i+2} are issued in turn when both can run.
     const auto s_mma = [&](int j, int kk) {
-      umma_f8(tmem + (uint32_t)((j & 1) * T::NS), sdesc_lo(base + (j % ST) * T::TILE, 16) + kk * 2, HI_KV,
+      umma_f8(tmem + (uint32_t)((j & 1) * T::NS), sdesc_lo(base + (j % KST) * T::TILE, 16) + kk * 2, HI_KV,
               q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
     };
     const auto pv_mma = [&](int i, int kk) {
-      umma_f8(tmem + T::O_COL + (i % NTG) * T::NO, sdesc_lo(base + T::OFF_V + (i % ST) * T::TILE, 16) + kk * (32 * HD / 16),
+      umma_f8(tmem + T::O_COL + (i % NTG) * T::NO, sdesc_lo(base + T::OFF_V + (i % VST) * T::TILE, 16) + kk * (32 * HD / 16),
               HI_KV, sdesc_lo(base + T::OFF_P + (i & 1) * T::P_BYTES, 128) + kk * 32, HI_P, IDESC_PV,
               kk > 0 || i >= NTG ? 1u : 0u);
     };
     constexpr int kS = HD / 32, kPV = kKeys / 32;
     if (tiles > 0) ok = wait(q_full, 0, kErrWaitOther);
     for (int j = 0; ok && j < min(2, tiles); ++j) {
-      ok = wait(&k_full[j % ST], (j / ST) & 1, kErrWaitFull);
+      ok = wait(&k_full[j % KST], (j / KST) & 1, kErrWaitFull);
       if (!ok) break;
       tc_fence_after();
       if (lead) {
 #pragma unroll
         for (int kk = 0; kk < kS; ++kk) s_mma(j, kk);
         umma_commit(&s_full[j & 1]);
-        umma_commit(&k_empty[j % ST]);
+        umma_commit(&k_empty[j % KST]);
       }
       __syncwarp();
     }
     for (int i = 0; ok && i < tiles; ++i) {
-      ok = wait(&v_full[i % ST], (i / ST) & 1, kErrWaitFull) && wait(&p_full[i & 1], (i >> 1) & 1, kErrWaitOther);
+      ok = wait(&v_full[i % VST], (i / VST) & 1, kErrWaitFull) && wait(&p_full[i & 1], (i >> 1) & 1, kErrWaitOther);
       if (!ok) break;
       const int j = i + 2;
-      uint64_t* jf = &k_full[j % ST];
-      const uint32_t jp = (j / ST) & 1;
+      uint64_t* jf = &k_full[j % KST];
+      const uint32_t jp = (j / KST) & 1;
       const bool both = j < tiles && __all_sync(0xffffffffu, mbar_test_wait(jf, jp));
       tc_fence_after();
       if (lead) {
@@ -406,10 +457,10 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
         }
         if (both) {
           umma_commit(&s_full[j & 1]);
-          umma_commit(&k_empty[j % ST]);
+          umma_commit(&k_empty[j % KST]);
         }
         umma_commit(&pv_done[i & 1]);
-        umma_commit(&v_empty[i % ST]);
+        umma_commit(&v_empty[i % VST]);
       }
       __syncwarp();
       if (j < tiles && !both) {
@@ -420,40 +471,32 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
 #pragma unroll
           for (int kk = 0; kk < kS; ++kk) s_mma(j, kk);
           umma_commit(&s_full[j & 1]);
-          umma_commit(&k_empty[j % ST]);
+          umma_commit(&k_empty[j % KST]);
         }
         __syncwarp();
       }
     }
   } else {
     // ---- queries: hi and lo codes, [16-byte chunk of hd][RT hi rows, RT lo rows][16]
-    constexpr int NQ = (RT + kSoftWarps - 1) / kSoftWarps;  // columns of a warp, all loads first
-    float x[NQ][HD / 32];
-    int tq[NQ], hq[NQ];
-#pragma unroll
-    for (int k = 0; k < NQ; ++k) {
-      const int c = warp + k * kSoftWarps, t = (r0 + c) / G, h = kh * G + (r0 + c) - t * G;
-      tq[k] = t;
-      hq[k] = h;
-      const bool live = c < RT && t >= t0 && t <= t1;
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + t) * a.ldq + (size_t)h * HD;
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) x[k][i] = live ? __bfloat162float(q[lane + 32 * i]) : 0.f;
-    }
 #pragma unroll
     for (int k = 0; k < NQ; ++k) {
       const int c = warp + k * kSoftWarps;
       if (c >= RT) break;
-      float m = 0.f;
+      const int t = tq[k], h = hq[k];
+      const bool live = t >= t0 && t <= t1;
+      float x[HD / 32], m = 0.f;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) m = fmaxf(m, x[k][i] - x[k][i] == 0.f ? fabsf(x[k][i]) : INFINITY);
+      for (int i = 0; i < HD / 32; ++i) {
+        x[i] = live ? __bfloat162float(xq[k][i]) : 0.f;
+        m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
+      }
       m = warp_max(m);
       const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
       const float s = bad ? 1.f : kv8_scale(m), rs = 1.f / s;  // powers of two
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
         const int e = lane + 32 * i;
-        const float y = bad ? 0.f : x[k][i] * rs;
+        const float y = bad ? 0.f : x[i] * rs;
         const uint32_t hi = e4m3x2(y, 0.f);
         const uint32_t lo = e4m3x2(y - e4m3x2_value(hi).x, 0.f);
         uint8_t* dst = smem + T::OFF_Q + (e / 16) * (T::NS * 16) + e % 16;
@@ -461,10 +504,11 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
         dst[(RT + c) * 16] = (uint8_t)lo;
       }
       if (lane == 0) {
-        const int t = tq[k], h = hq[k];
-        const bool live = t >= t0 && t <= t1;
         qf[c] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
-        for (int g = 0; g < NTG; ++g) refs[g * RT + c] = kNoRef;
+        for (int g = 0; g < NTG; ++g) {
+          refs[g * RT + c] = 0.f;
+          haves[g * RT + c] = 0.f;
+        }
         // a column without a query sees whatever there is; its output is zero, or none
         qhi[c] = live ? min(shift + t, k1 - 1) : k1 - 1;
         outs[c] = t >= a.seq ? -1 : (((int64_t)b * a.seq + t) * a.ldo + (int64_t)h * HD) * 2 + (live ? 1 : 0);
@@ -480,10 +524,11 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
     const int wg = warp >> 2, w4 = warp & 3, tg = wg / NCG, c0 = (wg % NCG) * CPW;
     const int key = 32 * w4 + lane;  // of the tile; this thread's TMEM lane
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16);
-    float* ref = refs + tg * RT + c0;
-    float* fac = facs + tg * RT + c0;
-    float* red = reinterpret_cast<float*>(smem + T::OFF_RED) + tg * 4 * RT + c0;
-    const auto pair = [](const float* p) { return *reinterpret_cast<const uint64_t*>(p); };
+    const uint32_t sm = smem_u32(smem);
+    const uint32_t ref = sm + T::OFF_REF + (tg * RT + c0) * 4, fac = sm + T::OFF_FAC + (tg * RT + c0) * 4;
+    const uint32_t have = sm + T::OFF_HAVE + (tg * RT + c0) * 4, red = sm + T::OFF_RED + (tg * 4 * RT + c0) * 4;
+    const uint32_t fq = sm + T::OFF_QF + c0 * 4;
+    bool known = false;  // every column has a reference
     uint64_t l2[CPW / 2];  // sums of the columns, in pairs
 #pragma unroll
     for (int c = 0; c < CPW / 2; ++c) l2[c] = 0ull;
@@ -492,22 +537,22 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
       // After a wait that gave up, the tiles are still walked (the waits return at once):
       // the warpgroup's barriers need every thread.
       ok = mbar_wait(&sc_full[i % T::SCALES], (i / T::SCALES) & 1, abort_flag, a.err, kErrWaitFull) && ok;
-      const float* sc = reinterpret_cast<const float*>(smem + T::OFF_SC + (i % T::SCALES) * 64);
+      const uint32_t sc = sm + T::OFF_SC + (i % T::SCALES) * 64 + (key >> 4) * 4;
       const bool on = kpos < k1;
-      const float ks = sc[key >> 4], vs = sc[8 + (key >> 4)];
+      const float ks = lds(sc), vs = lds(sc + 32);
       float ev;
       asm("lg2.approx.f32 %0, %1;" : "=f"(ev) : "f"(vs));
       const float inv = on && vs == vs ? __fdividef(1.f, vs) : 0.f;
       if (!on && c0 == 0) {  // rows past the context may hold NaN codes: 0 * NaN
-        ok = mbar_wait(&v_full[i % ST], (i / ST) & 1, abort_flag, a.err, kErrWaitFull) && ok;
-        uint8_t* row = smem + T::OFF_V + (i % ST) * T::TILE + key * HD;
+        ok = mbar_wait(&v_full[i % VST], (i / VST) & 1, abort_flag, a.err, kErrWaitFull) && ok;
+        const uint32_t row = sm + T::OFF_V + (i % VST) * T::TILE + key * HD;
 #pragma unroll 1
-        for (int x = 0; x < HD; x += 16) *reinterpret_cast<uint4*>(row + x) = make_uint4(0u, 0u, 0u, 0u);
+        for (int x = 0; x < HD; x += 16) sts4(row + x, 0u, 0u, 0u, 0u);
       }
       ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
       tc_fence_after();
-      // z of this key for the group's columns
-      float z[CPW];
+      // y of this key for the group's columns: z + bias - ref (ref = bias before the first)
+      float y[CPW];
       {
         uint32_t hi[CPW], lo[CPW];
         tmem_ld<CPW>(tl + (i & 1) * T::NS + c0, hi);
@@ -515,15 +560,20 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
         tmem_ld_wait();
         const uint64_t ks2 = f2pack(ks, ks), ev2 = f2pack(ev, ev);
 #pragma unroll
-        for (int c = 0; c < CPW; c += 2) {
-          const uint64_t s2 = fadd2(f2pack(__uint_as_float(hi[c]), __uint_as_float(hi[c + 1])),
-                                    f2pack(__uint_as_float(lo[c]), __uint_as_float(lo[c + 1])));
-          f2unpack(ffma2(s2, fmul2(ks2, pair(qf + c0 + c)), ev2), z[c], z[c + 1]);
+        for (int c = 0; c < CPW; c += 4) {
+          const float4 f4 = lds4(fq + c * 4), r4 = lds4(ref + c * 4);
+          const uint64_t f2[2] = {f2pack(f4.x, f4.y), f2pack(f4.z, f4.w)}, r2[2] = {f2pack(r4.x, r4.y), f2pack(r4.z, r4.w)};
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const uint64_t s2 = fadd2(f2pack(__uint_as_float(hi[c + e]), __uint_as_float(hi[c + e + 1])),
+                                      f2pack(__uint_as_float(lo[c + e]), __uint_as_float(lo[c + e + 1])));
+            f2unpack(ffma2(s2, fmul2(ks2, f2[e / 2]), fadd2(ev2, r2[e / 2])), y[c + e], y[c + e + 1]);
+          }
         }
       }
       if (ALIBI) {
 #pragma unroll
-        for (int c = 0; c < CPW; ++c) z[c] -= slope[c0 + c] * (float)(qhi[c0 + c] - kpos);
+        for (int c = 0; c < CPW; ++c) y[c] -= slope[c0 + c] * (float)(qhi[c0 + c] - kpos);
       }
       // some column's edge lies in the tile
       if (base + kKeys > qlo + 1 || (a.window > 0 && base <= k1 - 1 - a.window)) {
@@ -531,38 +581,53 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
 #pragma unroll
         for (int c = 0; c < CPW; ++c) {
           const int back = qhi[c0 + c] - kpos;
-          if (back < 0 || back >= w) z[c] = -INFINITY;
+          if (back < 0 || back >= w) y[c] = -INFINITY;
         }
       }
-      float top = -INFINITY;
+      float top = fmaxf(y[0], y[1]);
 #pragma unroll
-      for (int c = 0; c < CPW; c += 2) {
-        float u, w;
-        f2unpack(fadd2(f2pack(z[c], z[c + 1]), pair(ref + c)), u, w);
-        top = fmax3(top, u, w);
-      }
+      for (int c = 2; c < CPW; c += 2) top = fmax3(top, y[c], y[c + 1]);
       // P is free (and, with two tile groups, this group's O holds all its tiles)
       if (i >= 2) ok = mbar_wait(&pv_done[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
-      if (wg_any<NCG * NTG>(wg, top > kBias + kSlack)) {
+      if (wg_any<NCG * NTG>(wg, !known || top > kBias + kSlack)) {
         // new references: the maximum of every column over the tile's keys
 #pragma unroll
-        for (int c = 0; c < CPW; ++c) {
-          const float m = warp_max(z[c]);
-          if (lane == 0) red[w4 * RT + c] = m;
+        for (int c = 0; c < CPW; c += 4) {
+          const float4 r = lds4(ref + c * 4);
+          y[c] -= r.x;
+          y[c + 1] -= r.y;
+          y[c + 2] -= r.z;
+          y[c + 3] -= r.w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float m = warp_max(y[c + e]);
+            if (lane == 0) sts(red + (w4 * RT + c + e) * 4, m);
+          }
         }
         if (NTG == 1 && i > 0)
           ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
         tc_fence_after();
         wg_sync<NCG * NTG>(wg);
         if (key < CPW) {
-          const float m = fmaxf(fmaxf(red[key], red[RT + key]), fmaxf(red[2 * RT + key], red[3 * RT + key]));
-          const float was = ref[key], now = m == -INFINITY ? was : fminf(was, kBias - m);
-          fac[key] = was == kNoRef ? 1.f : fast_exp2(now - was);
-          ref[key] = now;
+          const uint32_t at = red + key * 4;
+          const float m = fmaxf(fmaxf(lds(at), lds(at + RT * 4)), fmaxf(lds(at + 2 * RT * 4), lds(at + 3 * RT * 4)));
+          const float was = lds(ref + key * 4);
+          const bool first = lds(have + key * 4) == 0.f;
+          float now = was;  // a column whose keys are all masked stays without
+          if (m != -INFINITY) {
+            now = first ? kBias - m : fminf(was, kBias - m);
+            sts(have + key * 4, 1.f);
+          }
+          sts(fac + key * 4, first ? 1.f : fast_exp2(now - was));
+          sts(ref + key * 4, now);
         }
         wg_sync<NCG * NTG>(wg);
 #pragma unroll
-        for (int c = 0; c < CPW; c += 2) l2[c / 2] = fmul2(l2[c / 2], pair(fac + c));
+        for (int c = 0; c < CPW; c += 4) {
+          const float4 f = lds4(fac + c * 4);
+          l2[c / 2] = fmul2(l2[c / 2], f2pack(f.x, f.y));
+          l2[c / 2 + 1] = fmul2(l2[c / 2 + 1], f2pack(f.z, f.w));
+        }
         if (i >= NTG) {
 #pragma unroll 1
           for (int term = 0; term < 3; ++term) {
@@ -571,50 +636,59 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
             tmem_ld<CPW>(at, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < CPW; c += 2) {
-              float u, w;
-              f2unpack(fmul2(f2pack(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), pair(fac + c)), u, w);
-              o[c] = __float_as_uint(u);
-              o[c + 1] = __float_as_uint(w);
+            for (int c = 0; c < CPW; c += 4) {
+              const float4 f = lds4(fac + c * 4);
+              o[c] = __float_as_uint(__uint_as_float(o[c]) * f.x);
+              o[c + 1] = __float_as_uint(__uint_as_float(o[c + 1]) * f.y);
+              o[c + 2] = __float_as_uint(__uint_as_float(o[c + 2]) * f.z);
+              o[c + 3] = __float_as_uint(__uint_as_float(o[c + 3]) * f.w);
             }
             tmem_st<CPW>(at, o);
           }
           tmem_st_wait();
         }
+        known = __all_sync(0xffffffffu, lds(have + (lane % CPW) * 4) != 0.f);
+#pragma unroll
+        for (int c = 0; c < CPW; c += 4) {
+          const float4 r = lds4(ref + c * 4);
+          y[c] += r.x;
+          y[c + 1] += r.y;
+          y[c + 2] += r.z;
+          y[c + 3] += r.w;
+        }
       }
       // probabilities, and their three codes: chunks of 16 columns (of 8 + 8 when RT = 8)
       const uint64_t inv2 = f2pack(inv, inv);
+      const __half2 eight = __float2half2_rn(8.f);
       uint32_t code[3][CPW / 4];
 #pragma unroll
       for (int c = 0; c < CPW; c += 4) {
         float p[4];
-        f2unpack(fadd2(f2pack(z[c], z[c + 1]), pair(ref + c)), p[0], p[1]);
-        f2unpack(fadd2(f2pack(z[c + 2], z[c + 3]), pair(ref + c + 2)), p[2], p[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = fast_exp2(p[e]);
+        for (int e = 0; e < 4; ++e) p[e] = fast_exp2(y[c + e]);
         l2[c / 2] = ffma2(f2pack(p[0], p[1]), inv2, l2[c / 2]);
         l2[c / 2 + 1] = ffma2(f2pack(p[2], p[3]), inv2, l2[c / 2 + 1]);
         __half2 u = __floats2half2_rn(p[0], p[1]), w = __floats2half2_rn(p[2], p[3]);
 #pragma unroll
         for (int term = 0; term < 3; ++term) {
-          const uint32_t cu = e5m2x2(u), cw = e5m2x2(w);
-          code[term][c / 4] = cu | (cw << 16);
-          if (term < 2) {  // exact: the remainder has fewer bits than FP16 holds
-            u = __hsub2(u, e5m2x2_value(cu));
-            w = __hsub2(w, e5m2x2_value(cw));
+          const uint32_t four = e5m2x4(u, w);
+          code[term][c / 4] = four;
+          if (term < 2) {  // 8 (u - code), exact: the remainder has fewer bits than FP16 holds
+            u = __hmul2(__hsub2(u, e5m2_lo(four)), eight);
+            w = __hmul2(__hsub2(w, e5m2_hi(four)), eight);
           }
         }
       }
-      uint8_t* pt = smem + T::OFF_P + (i & 1) * T::P_BYTES + key * 16;
+      const uint32_t pt = sm + T::OFF_P + (i & 1) * T::P_BYTES + key * 16;
       if constexpr (RT == 8) {
-        st_shared_v4(pt, code[0][0], code[0][1], code[1][0], code[1][1]);
-        st_shared_v4(pt + kKeys * 16, code[2][0], code[2][1], 0u, 0u);
+        sts4(pt, code[0][0], code[0][1], code[1][0], code[1][1]);
+        sts4(pt + kKeys * 16, code[2][0], code[2][1], 0u, 0u);
       } else {
 #pragma unroll
         for (int term = 0; term < 3; ++term)
 #pragma unroll
           for (int x = 0; x < CPW / 16; ++x)
-            st_shared_v4(pt + ((term * RT + c0) / 16 + x) * (kKeys * 16), code[term][4 * x], code[term][4 * x + 1],
+            sts4(pt + ((term * RT + c0) / 16 + x) * (kKeys * 16), code[term][4 * x], code[term][4 * x + 1],
                          code[term][4 * x + 2], code[term][4 * x + 3]);
       }
       fence_proxy_async_smem();
@@ -630,125 +704,136 @@ __global__ void __launch_bounds__(KT<HD, RT, DEEP>::THREADS, KT<HD, RT, DEEP>::P
       if (c & 1) v = w;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) red[w4 * RT + c] = v;
+      if (lane == 0) sts(red + (w4 * RT + c) * 4, v);
     }
     wg_sync<NCG * NTG>(wg);
-    if (key < CPW) lsum[tg * RT + c0 + key] = (red[key] + red[RT + key]) + (red[2 * RT + key] + red[3 * RT + key]);
+    if (key < CPW) {
+      const uint32_t at = red + key * 4;
+      lsum[tg * RT + c0 + key] = (lds(at) + lds(at + RT * 4)) + (lds(at + 2 * RT * 4) + lds(at + 3 * RT * 4));
+    }
     // every PV has completed (the last two cover the others: MMAs finish in order)
     for (int i = max(0, tiles - 2); i < tiles; ++i)
       ok = mbar_wait(&pv_done[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
     tc_fence_after();
-    soft_sync<kSoftWarps>();
-
-    // ---- O^T -> part [column][dim] over the stages; the tile groups are joined, in
-    // group order. From here on the code runs once, so it is kept short: fetching it
-    // costs more than running it.
-    if (threadIdx.x < RT) {
-      const int c = threadIdx.x;
-      float r = refs[c], den = lsum[c];
-      facs[c] = 1.f;
-      if constexpr (NTG == 2) {
-        r = fminf(r, refs[RT + c]);
-        const float f0 = fast_exp2(r - refs[c]), f1 = fast_exp2(r - refs[RT + c]);
-        facs[c] = f0;
-        facs[RT + c] = f1;
-        den = f0 * den + f1 * lsum[RT + c];
-      }
-      refs[c] = r;
-      // the weight of the CTA's own sums when the context is not split
-      lsum[c] = splits > 1 ? den : den == 0.f ? 0.f : 1.f / den;
-    }
-    soft_sync<kSoftWarps>();
-    float* part = reinterpret_cast<float*>(smem);
-    if (warp < NCG * 4) {
-      // lane = dim (head_dim 64: 16 lanes of every warp)
-      const int dim = HD == 128 ? 32 * w4 + lane : 16 * w4 + lane;
-#pragma unroll 1
-      for (int c = c0; c < c0 + CPW; c += 8) {
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = 0.f;
-#pragma unroll 1
-        for (int g = 0; g < min(NTG, tiles); ++g)
-#pragma unroll 1
-          for (int term = 0; term < 3; ++term) {
-            uint32_t x[8];
-            tmem_ld<8>(tl + T::O_COL + g * T::NO + term * RT + c, x);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = fmaf(facs[g * RT + c + e], __uint_as_float(x[e]), o[e]);
-          }
-        if (HD == 128 || lane < 16) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) part[(c + e) * HD + dim] = o[e];
-        }
-      }
-    }
-    tc_fence_before();
   }
   // A bounded wait that gave up is in the error word: every thread still takes the
   // barriers below, and the outputs are not written.
   ok = __syncthreads_and(ok ? 1 : 0) != 0;
-  if (warp == kSoftWarps) tmem_dealloc(tmem, T::TMEM);
 
-  float* part = reinterpret_cast<float*>(smem);
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
-  if (splits == 1) {
-    for (int idx = threadIdx.x; ok && idx < RT * HD; idx += T::THREADS) {
-      const int c = idx / HD;
-      const int64_t to = outs[c];
-      if (to < 0) break;
-      out[(to >> 1) + idx % HD] = __float2bfloat16_rn(to & 1 ? part[idx] * lsum[c] : 0.f);
-    }
-    return;
-  }
-  // ---- the splits of a context are joined in rank order: 2^(ref_s - ref) of every
-  // split's O and l; (column, dim) pairs are dealt out over the cluster.
-  float* pr = reinterpret_cast<float*>(smem + T::OFF_P);  // [split][RT] references
-  float* pl = pr + kMaxCluster * RT;                      // sums
-  float* pw = pl + kMaxCluster * RT;                      // weights
-  cluster_sync();
-  for (int i = threadIdx.x; i < splits * RT; i += T::THREADS) {
-    pr[i] = ld_peer(peer_addr(&refs[i % RT], i / RT));
-    pl[i] = ld_peer(peer_addr(&lsum[i % RT], i / RT));
-  }
-  __syncthreads();
+  // ---- joining. The tile groups, in group order, then the splits of the context, in
+  // rank order: every CTA of the cluster owns a piece of the [column][dim] outputs, and
+  // the others write their part of it, unnormalised, with references and sums, into its
+  // shared memory. This code runs once and is kept short: fetching it costs more than
+  // running it.
   if (threadIdx.x < RT) {
-    float r = kNoRef, den = 0.f;
-    for (int s = 0; s < splits; ++s) r = fminf(r, pr[s * RT + threadIdx.x]);
-    for (int s = 0; s < splits; ++s) den = fmaf(fast_exp2(r - pr[s * RT + threadIdx.x]), pl[s * RT + threadIdx.x], den);
-    for (int s = 0; s < splits; ++s)
-      pw[s * RT + threadIdx.x] = den == 0.f ? 0.f : fast_exp2(r - pr[s * RT + threadIdx.x]) / den;
+    const int c = threadIdx.x;
+    float r = haves[c] != 0.f ? refs[c] : kNoRef, den = lsum[c];
+    facs[c] = 1.f;
+    if constexpr (NTG == 2) {
+      const float r0g = r, r1g = haves[RT + c] != 0.f ? refs[RT + c] : kNoRef;
+      r = fminf(r0g, r1g);
+      facs[c] = fast_exp2(r - r0g);
+      facs[RT + c] = fast_exp2(r - r1g);
+      den = facs[c] * den + facs[RT + c] * lsum[RT + c];
+    }
+    refs[c] = r;
+    lsum[c] = den;
   }
+  if (splits > 1) cluster_wait();  // every CTA of the cluster has started
   __syncthreads();
-  for (int idx = split * T::THREADS + threadIdx.x; ok && idx < RT * HD; idx += splits * T::THREADS) {
-    const int c = idx / HD;
+  const int piece = RT * HD / splits, cols = max(1, piece / HD);  // of one owner (powers of two)
+  const int lp = 31 - __clz(piece), lc = 31 - __clz(cols);
+  const float* in = reinterpret_cast<const float*>(smem + T::OFF_IN);
+  const float2* inl = reinterpret_cast<const float2*>(smem + T::OFF_INL);
+  if ((int)threadIdx.x < splits * cols) {
+    const int to = (int)threadIdx.x >> lc, k = (int)threadIdx.x & (cols - 1), c = (to << lp) / HD + k;
+    st_peer2(peer_addr(inl + split * cols + k, to), refs[c], lsum[c]);
+  }
+  if (warp < NCG * 4) {
+    // lane = dim (head_dim 64: 16 lanes of every warp), a column group per warpgroup
+    const int w4 = warp & 3, c0 = (warp >> 2) * CPW;
+    const int dim = HD == 128 ? 32 * w4 + lane : 16 * w4 + lane;
+    const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + T::O_COL;
+#pragma unroll 1
+    for (int c = c0; c < c0 + CPW; c += 8) {
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll 1
+      for (int x = 0; x < 3 * min(NTG, tiles); ++x) {  // group x / 3, term x % 3
+        const float unit = x % 3 == 0 ? 1.f : x % 3 == 1 ? 0.125f : 0.015625f;
+        uint32_t v[8];
+        tmem_ld<8>(tl + (x / 3) * T::NO + (x % 3) * RT + c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(facs[(x / 3) * RT + c + e] * unit, __uint_as_float(v[e]), o[e]);
+      }
+      if (HD == 128 || lane < 16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int idx = (c + e) * HD + dim;
+          st_peer(peer_addr(in + (split << lp) + (idx & (piece - 1)), idx >> lp), o[e]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  if (splits > 1) cluster_sync();
+  else __syncthreads();
+  if (warp == kSoftWarps) tmem_dealloc(tmem, T::TMEM);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
+  const int first = split * piece / HD;
+  for (int idx = threadIdx.x; ok && idx < piece; idx += T::THREADS) {
+    const int e = split * piece + idx, c = e / HD;
     const int64_t to = outs[c];
     if (to < 0) break;
-    float v = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) v = fmaf(pw[s * RT + c], ld_peer(peer_addr(part + idx, s)), v);
-    out[(to >> 1) + idx % HD] = __float2bfloat16_rn(to & 1 ? v : 0.f);
+    float ref = kNoRef, num = 0.f, den = 0.f;
+    for (int s = 0; s < splits; ++s) ref = fminf(ref, inl[s * cols + c - first].x);
+    for (int s = 0; s < splits; ++s) {
+      const float2 rl = inl[s * cols + c - first];
+      const float f = fast_exp2(ref - rl.x);
+      num = fmaf(f, in[s * piece + idx], num);
+      den = fmaf(f, rl.y, den);
+    }
+    out[(to >> 1) + e % HD] = __float2bfloat16_rn((to & 1) && den != 0.f ? num / den : 0.f);
   }
-  cluster_sync();  // no CTA leaves while another reads its partials
 }
 
-template <int HD, int RT, bool DEEP>
+// Share of the SMs' CTAs, in thousandths, that run at once in clusters of 2^k: a cluster
+// has to fit the SMs of one GPC. From cudaOccupancyMaxActiveClusters on kernels of the
+// same threads and shared memory (148, 148, 132, 120, 112 CTAs with one to an SM; 296,
+// 296, 284, 264, 224 with two); for a kernel with TMEM the runtime counts one CTA an SM.
+constexpr int kMaxLog = 4;
+static_assert(1 << kMaxLog == kMaxCluster, "");
+constexpr int kResident[2][kMaxLog + 1] = {{1000, 1000, 891, 810, 756}, {1000, 1000, 940, 880, 756}};
+
+template <int HD, int RT, bool ALIBI>
 cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
-  using T = KT<HD, RT, DEEP>;
+  using T = KT<HD, RT>;
+  auto kern = kv8_attn_kernel<HD, RT, ALIBI>;
+  static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_release);
+  }
   const int group = a.heads / a.c.kv_heads;
   const int64_t row_tiles = ((int64_t)a.seq * group + RT - 1) / RT;
   const int64_t pairs = row_tiles * a.c.kv_heads * a.batch;
-  // One wave of resident CTAs: a context is split while the grid leaves SMs idle, down
-  // to one 128-key tile a CTA.
+  // A context is split while every cluster is resident at once and a CTA has a tile:
+  // 8 pairs of 32768 keys (head_dim 128) take 179 us unsplit, 28 in clusters of 8, 19 in
+  // clusters of 16; 128 pairs of 4096 keys (head_dim 64) 28, and 17 in clusters of 4;
+  // 512 pairs of them 48, and 52 in clusters of 2, which no longer fit at once.
   const int keys = a.window > 0 ? std::min(a.max_ctx, a.window + a.seq + kKv8Page) : a.max_ctx;
-  int splits = 1;
-  while (splits < kMaxCluster && pairs * splits * 2 <= (int64_t)a.sm_count * T::PER_SM && splits * 2 * kKeys <= keys) splits *= 2;
-  if (getenv("WVT_S")) splits = atoi(getenv("WVT_S"));
-  auto kern = a.alibi ? kv8_attn_kernel<HD, RT, DEEP, true> : kv8_attn_kernel<HD, RT, DEEP, false>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
-  if (e == cudaSuccess && splits > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return e;
+  const int64_t slots = (int64_t)a.sm_count * T::PER_SM;
+  int k = 0;
+  while (k < kMaxLog && pairs << (k + 1) <= slots * kResident[T::PER_SM > 1][k + 1] / 1000 && (kKeys << (k + 1)) <= keys) ++k;
+  const int splits = 1 << k;
   cudaLaunchConfig_t lc{};
   lc.gridDim = dim3((unsigned)(row_tiles * splits), a.c.kv_heads, a.batch);
   lc.blockDim = dim3(T::THREADS);
@@ -759,8 +844,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnAr
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = splits;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = 1;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   lc.attrs = at;
   lc.numAttrs = splits > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&lc, kern, mk, mv, a, splits);
@@ -768,11 +852,14 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnAr
 
 template <int HD> cudaError_t launch_hd(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.seq * (a.heads / a.c.kv_heads);
-  const bool deep = getenv("WVT_D") && atoi(getenv("WVT_D"));
-  if (rows <= 8) return deep ? launch<HD, 8, true>(mk, mv, a, s) : launch<HD, 8, false>(mk, mv, a, s);
-  if (rows <= 16) return deep ? launch<HD, 16, true>(mk, mv, a, s) : launch<HD, 16, false>(mk, mv, a, s);
-  if (rows <= 32) return launch<HD, 32, false>(mk, mv, a, s);
-  return launch<HD, 64, false>(mk, mv, a, s);
+  const auto go = [&](auto alibi) {
+    constexpr bool A = decltype(alibi)::value;
+    if (rows <= 8) return launch<HD, 8, A>(mk, mv, a, s);
+    if (rows <= 16) return launch<HD, 16, A>(mk, mv, a, s);
+    if (rows <= 32) return launch<HD, 32, A>(mk, mv, a, s);
+    return launch<HD, 64, A>(mk, mv, a, s);
+  };
+  return a.alibi ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace
