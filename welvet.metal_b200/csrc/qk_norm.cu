@@ -86,38 +86,39 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rows_kernel(const Q
   }
 }
 
-// A CTA's sums of the gamma gradients into its two rows of `partial` (queries, keys):
-// acc [warps][2][head_dim] is added up in warp order.
+// A CTA's sum of its side's gamma gradient into its row of `partial`: acc
+// [warps][head_dim] is added up in warp order.
 WV_DEV void write_partial(const QkNormArgs& a, const float* acc) {
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * a.head_dim; i += blockDim.x) {
+  for (int i = threadIdx.x; i < a.head_dim; i += blockDim.x) {
     float s = 0.f;
-    for (int w = 0; w < kWarpsPerCta; ++w) s += acc[w * 2 * a.head_dim + i];
-    a.partial[(size_t)blockIdx.x * 2 * a.head_dim + i] = s;
+    for (int w = 0; w < kWarpsPerCta; ++w) s += acc[w * a.head_dim + i];
+    a.partial[(size_t)blockIdx.x * a.head_dim + i] = s;
   }
 }
 
-// Backward with the same mapping. The gamma gradients are summed in registers over a
-// warp's rows, over the CTA's warps in shared memory, and over the CTAs by
-// dgamma_kernel, each time in a fixed order: no atomics, the same bits every time.
+// Backward with the same mapping. The first part_q CTAs take the query rows, the others
+// the key rows. The gamma gradients are summed in registers over a warp's rows, over
+// the CTA's warps in shared memory, and over the CTAs by dgamma_kernel, each time in a
+// fixed order: no atomics, the same bits every time.
 template <class T>
-__global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rows_bwd_kernel(const QkNormArgs a) {
+__global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rows_bwd_kernel(const QkNormArgs a, int part_q) {
   pdl_wait();
   pdl_trigger();
-  extern __shared__ float acc[];  // [warps][2][head_dim]
+  extern __shared__ float acc[];  // [warps][head_dim]
   const int half = a.head_dim / 2, lane = (int)lane_id(), warp = (int)warp_id();
-  const int per = a.heads + a.kv_heads;
-  const int64_t rows = a.tokens * per;
-  float ga[2][kMaxPairs] = {}, gb[2][kMaxPairs] = {};
-  for (int64_t row = (int64_t)blockIdx.x * kWarpsPerCta + warp; row < rows; row += (int64_t)gridDim.x * kWarpsPerCta) {
+  const bool key = (int)blockIdx.x >= part_q;
+  const int per = key ? a.kv_heads : a.heads;
+  const int64_t rows = a.tokens * per, ctas = key ? gridDim.x - part_q : part_q;
+  const float* gamma = key ? a.k_gamma : a.q_gamma;
+  float ga[kMaxPairs] = {}, gb[kMaxPairs] = {};
+  for (int64_t row = (int64_t)(blockIdx.x - (key ? part_q : 0)) * kWarpsPerCta + warp; row < rows;
+       row += ctas * kWarpsPerCta) {
     const int64_t t = row / per;
-    const int hh = (int)(row % per);
-    const bool key = hh >= a.heads;
-    const size_t h = (size_t)(key ? hh - a.heads : hh) * a.head_dim;
+    const size_t h = (size_t)(row % per) * a.head_dim;
     const T* x = static_cast<const T*>(key ? a.k : a.q) + (size_t)t * (key ? a.ldk : a.ldq) + h;
     const T* dy = static_cast<const T*>(key ? a.dk_out : a.dq_out) + (size_t)t * (key ? a.lddko : a.lddqo) + h;
     T* dx = static_cast<T*>(key ? a.k_out : a.q_out) + (size_t)t * (key ? a.ldko : a.ldqo) + h;
-    const float* gamma = key ? a.k_gamma : a.q_gamma;
     const float2* cs = angles(a, t, half);
     float xa[kMaxPairs], xb[kMaxPairs], za[kMaxPairs], zb[kMaxPairs], ss = 0.f, dot = 0.f;
 #pragma unroll
@@ -143,11 +144,8 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rows_bwd_kernel(con
         if (i >= half) continue;
         xa[j] *= r;
         xb[j] *= r;
-        const float pa = za[j] * xa[j], pb = zb[j] * xb[j];
-        ga[0][j] += key ? 0.f : pa;
-        gb[0][j] += key ? 0.f : pb;
-        ga[1][j] += key ? pa : 0.f;
-        gb[1][j] += key ? pb : 0.f;
+        ga[j] += za[j] * xa[j];
+        gb[j] += zb[j] * xb[j];
         za[j] *= gamma[i];
         zb[j] *= gamma[half + i];
         dot += za[j] * xa[j] + zb[j] * xb[j];
@@ -163,70 +161,89 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rows_bwd_kernel(con
     }
   }
 #pragma unroll
-  for (int side = 0; side < 2; ++side)
-#pragma unroll
-    for (int j = 0; j < kMaxPairs; ++j) {
-      const int i = lane + 32 * j;
-      if (i < half) {
-        acc[(warp * 2 + side) * a.head_dim + i] = ga[side][j];
-        acc[(warp * 2 + side) * a.head_dim + half + i] = gb[side][j];
-      }
+  for (int j = 0; j < kMaxPairs; ++j) {
+    const int i = lane + 32 * j;
+    if (i < half) {
+      acc[warp * a.head_dim + i] = ga[j];
+      acc[warp * a.head_dim + half + i] = gb[j];
     }
+  }
   write_partial(a, acc);
 }
 
-// dgamma = sum of the CTAs' partial rows: 32 columns a CTA, 32 threads on a column take
-// every 32nd row, then add up in row order.
-__global__ void __launch_bounds__(1024) dgamma_kernel(const float* partial, int parts, int hd, float* dq_gamma, float* dk_gamma) {
+// dgamma = sum of the CTAs' partial rows (the first part_q belong to the queries): 32
+// columns a CTA, 32 threads on a column take every 32nd row, then add up in row order.
+__global__ void __launch_bounds__(1024) dgamma_kernel(const float* partial, int part_q, int parts, int hd, float* dq_gamma,
+                                                      float* dk_gamma) {
   __shared__ float sum[32][33];
   pdl_wait();
   pdl_trigger();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, i = blockIdx.x * 32 + x;
+  const int to = blockIdx.y ? parts : part_q;
   float s = 0.f;
-  if (i < 2 * hd)
-    for (int p = y; p < parts; p += 32) s += partial[(size_t)p * 2 * hd + i];
+  if (i < hd)
+    for (int p = (blockIdx.y ? part_q : 0) + y; p < to; p += 32) s += partial[(size_t)p * hd + i];
   sum[y][x] = s;
   __syncthreads();
-  if (y == 0 && i < 2 * hd) {
+  if (y == 0 && i < hd) {
     for (int k = 1; k < 32; ++k) s += sum[k][x];
-    float* out = i < hd ? dq_gamma : dk_gamma;
-    if (out) out[i % hd] = s;
+    float* out = blockIdx.y ? dk_gamma : dq_gamma;
+    if (out) out[i] = s;
   }
 }
 
-// ------------------------------------------------------------ 16-byte rows
-// head_dim 64, 128, 256 with rows aligned to 16 bytes: VEC pairs of a row per lane (16
-// bytes of each half), so a row takes hd / 2 / VEC lanes and a warp RPW rows at once;
-// the partners of a rotation sit in one lane, and a warp keeps the angles and gammas of
-// its token in registers over all heads of its share. Bound by HBM: the loads of two
-// row groups are in flight before the first is used.
-template <class T, int HD> struct VT {
-  static constexpr int VEC = 16 / (int)sizeof(T), LPR = HD / 2 / VEC, RPW = 32 / LPR;
+// ------------------------------------------------------------ aligned rows
+// head_dim 64, 128, 256 with rows aligned to 16 bytes: VEC pairs of a row per lane, so a
+// row takes hd / 2 / VEC lanes and a warp RPW rows at once; the partners of a rotation
+// sit in one lane, and a warp keeps the angles of its token and the gammas of its side
+// in registers over all heads of its share. Bound by HBM: two groups of rows are
+// requested before the first is used. Forward: 16 bytes a load (16384 tokens x 64 heads
+// of 128, BF16: 92 us, 0.91 of the copy rate). Backward: four pairs a lane, since x,
+// dy, gamma, its gradient and the angles of eight pairs take 161 registers, 8 warps an
+// SM: 143 us for 16384 x 40 heads of 128, against 103 (0.76 of the copy rate).
+template <class T, int HD, bool BWD> struct VT {
+  static constexpr int VEC = BWD ? 4 : 16 / (int)sizeof(T), LPR = HD / 2 / VEC, RPW = 32 / LPR;
 };
-template <class T, int HD> WV_DEV float row_sum(float v) {
+template <int LPR> WV_DEV float row_sum(float v) {
 #pragma unroll
-  for (int o = VT<T, HD>::LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-WV_DEV void unpack(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+template <int WORDS> struct Raw {  // WORDS 32-bit words, loaded and stored at once
+  uint32_t w[WORDS];
+};
+template <int WORDS> WV_DEV void load_raw(Raw<WORDS>& r, const void* p) {
+  if constexpr (WORDS == 4) {
+    const uint4 v = *static_cast<const uint4*>(p);
+    r.w[0] = v.x;
+    r.w[1] = v.y;
+    r.w[2] = v.z;
+    r.w[3] = v.w;
+  } else {
+    const uint2 v = *static_cast<const uint2*>(p);
+    r.w[0] = v.x;
+    r.w[1] = v.y;
   }
 }
-WV_DEV void unpack(const uint4& u, float (&f)[4]) {
-  f[0] = __uint_as_float(u.x);
-  f[1] = __uint_as_float(u.y);
-  f[2] = __uint_as_float(u.z);
-  f[3] = __uint_as_float(u.w);
+template <int WORDS> WV_DEV void store_raw(void* p, const Raw<WORDS>& r) {
+  if constexpr (WORDS == 4) *static_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  else *static_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
 }
-WV_DEV uint4 pack(const float (&f)[8]) {
-  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+template <class T, int VEC> WV_DEV void unpack(const Raw<VEC * sizeof(T) / 4>& r, float (&f)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    f[i] = sizeof(T) == 4 ? __uint_as_float(r.w[i]) : __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
 }
-WV_DEV uint4 pack(const float (&f)[4]) {
-  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+template <class T, int VEC> WV_DEV Raw<VEC * sizeof(T) / 4> pack(const float (&f)[VEC]) {
+  Raw<VEC * sizeof(T) / 4> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) r.w[i / 2] = pack_bf16x2(f[i], f[i + 1]);
+  }
+  return r;
 }
 template <int N> WV_DEV void load_f(const float* p, float (&f)[N]) {
 #pragma unroll
@@ -239,27 +256,40 @@ template <int N> WV_DEV void load_f(const float* p, float (&f)[N]) {
   }
 }
 
-// A warp's share of one token: groups [g0, g1) of RPW heads, the query groups first.
-// BWD: dx and the gamma gradients instead of y.
+// A warp's share of one token and side: groups of RPW heads. The first part_q CTAs take
+// the queries, the others the keys; slices_q / slices_k warps share a token. BWD: dx and
+// the gamma gradients instead of y.
 template <class T, int HD, bool BWD>
-__global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_vec_kernel(const QkNormArgs a, int slices) {
-  using V = VT<T, HD>;
-  constexpr int VEC = V::VEC;
+__global__ void __launch_bounds__(kWarpsPerCta * 32, BWD ? 4 : 3)
+    qk_norm_vec_kernel(const QkNormArgs a, int part_q, int slices_q, int slices_k) {
+  using V = VT<T, HD, BWD>;
+  constexpr int VEC = V::VEC, WORDS = VEC * (int)sizeof(T) / 4;
   extern __shared__ float acc[];
   pdl_wait();
   pdl_trigger();
   const int lane = (int)lane_id(), warp = (int)warp_id();
   const int sub = lane / V::LPR, at = (lane % V::LPR) * VEC;  // row of the group, first pair
-  const int gq = (a.heads + V::RPW - 1) / V::RPW, groups = gq + (a.kv_heads + V::RPW - 1) / V::RPW;
-  const int per = (groups + slices - 1) / slices;
-  const uint32_t units = (uint32_t)a.tokens * (uint32_t)slices;
-  float dg[BWD ? 2 : 1][2][VEC];  // [queries, keys][half]
+  const bool key = (int)blockIdx.x >= part_q;
+  const int heads = key ? a.kv_heads : a.heads;
+  const uint32_t slices = key ? slices_k : slices_q, ctas = key ? gridDim.x - part_q : part_q;
+  const int groups = (heads + V::RPW - 1) / V::RPW, per = (groups + (int)slices - 1) / (int)slices;
+  const uint32_t units = heads ? (uint32_t)a.tokens * slices : 0u;
+  const float* gamma = key ? a.k_gamma : a.q_gamma;
+  const T* xp = static_cast<const T*>(key ? a.k : a.q) + at;
+  const T* dyp = BWD ? static_cast<const T*>(key ? a.dk_out : a.dq_out) + at : nullptr;
+  T* yp = static_cast<T*>(key ? a.k_out : a.q_out) + at;
+  const int64_t ldx = key ? a.ldk : a.ldq, lddy = key ? a.lddko : a.lddqo, ldy = key ? a.ldko : a.ldqo;
+  float w[2][VEC], dg[2][VEC];
 #pragma unroll
-  for (int i = 0; i < (BWD ? 2 : 1) * 2 * VEC; ++i) (&dg[0][0][0])[i] = 0.f;
+  for (int i = 0; i < VEC; ++i) w[0][i] = w[1][i] = dg[0][i] = dg[1][i] = 0.f;
+  if (gamma) {
+    load_f(gamma + at, w[0]);
+    load_f(gamma + HD / 2 + at, w[1]);
+  }
 
-  for (uint32_t unit = blockIdx.x * kWarpsPerCta + warp; unit < units; unit += gridDim.x * kWarpsPerCta) {
-    const int64_t t = unit / (uint32_t)slices;
-    const int g0 = (int)(unit % (uint32_t)slices) * per, g1 = min(groups, g0 + per);
+  for (uint32_t unit = (blockIdx.x - (key ? part_q : 0)) * kWarpsPerCta + warp; unit < units; unit += ctas * kWarpsPerCta) {
+    const int64_t t = unit / slices;
+    const int g0 = (int)(unit % slices) * per, g1 = min(groups, g0 + per);
     float cs[2 * VEC];
     const float2* tab = angles(a, t, HD / 2);
     if (tab) {
@@ -271,106 +301,93 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_vec_kernel(const Qk
         cs[2 * i + 1] = 0.f;
       }
     }
-    auto side = [&](int key, const void* xp, int64_t ldx, const void* dyp, int64_t lddy, void* yp, int64_t ldy,
-                    const float* gamma, int heads, int from, int to) {
-      if (from >= to) return;
-      const T* x = static_cast<const T*>(xp) + t * ldx + at;
-      const T* dy = BWD ? static_cast<const T*>(dyp) + t * lddy + at : nullptr;
-      T* y = static_cast<T*>(yp) + t * ldy + at;
-      float w[2][VEC];
-      if (gamma) {
-        load_f(gamma + at, w[0]);
-        load_f(gamma + HD / 2 + at, w[1]);
-      }
-      constexpr int U = 2;  // row groups in flight
-      for (int g = from; g < to; g += U) {
-        uint4 in[U][2], up[U][2];
+    const T* x = xp + t * ldx;
+    const T* dy = BWD ? dyp + t * lddy : nullptr;
+    T* y = yp + t * ldy;
+    constexpr int U = BWD && sizeof(T) == 4 ? 1 : 2;  // row groups in flight (FP32 backward: 27 us with 2, 22 with 1)
+    for (int g = g0; g < g1; g += U) {
+      Raw<WORDS> in[U][2], up[BWD ? U : 1][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = (g + u) * V::RPW + sub;
-          const bool on = g + u < to && h < heads;
-          in[u][0] = in[u][1] = up[u][0] = up[u][1] = make_uint4(0u, 0u, 0u, 0u);
-          if (on && (!BWD || gamma)) {
-            in[u][0] = *reinterpret_cast<const uint4*>(x + (size_t)h * HD);
-            in[u][1] = *reinterpret_cast<const uint4*>(x + (size_t)h * HD + HD / 2);
-          }
-          if (BWD && on) {
-            up[u][0] = *reinterpret_cast<const uint4*>(dy + (size_t)h * HD);
-            up[u][1] = *reinterpret_cast<const uint4*>(dy + (size_t)h * HD + HD / 2);
-          }
-        }
+      for (int u = 0; u < U; ++u) {
+        const int h = (g + u) * V::RPW + sub;
+        const bool on = g + u < g1 && h < heads;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = (g + u) * V::RPW + sub;
-          float xa[VEC], xb[VEC], ya[VEC], yb[VEC], r = 1.f;
-          unpack(in[u][0], xa);
-          unpack(in[u][1], xb);
-          if (gamma) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) ss += xa[i] * xa[i] + xb[i] * xb[i];
-            r = rsqrtf(row_sum<T, HD>(ss) * (1.f / HD) + a.eps);
-          }
-          if (!BWD) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float za = gamma ? xa[i] * r * w[0][i] : xa[i], zb = gamma ? xb[i] * r * w[1][i] : xb[i];
-              ya[i] = za * cs[2 * i] - zb * cs[2 * i + 1];
-              yb[i] = za * cs[2 * i + 1] + zb * cs[2 * i];
-            }
-          } else {
-            float da[VEC], db[VEC], dot = 0.f;
-            unpack(up[u][0], da);
-            unpack(up[u][1], db);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              float za = da[i] * cs[2 * i] + db[i] * cs[2 * i + 1], zb = db[i] * cs[2 * i] - da[i] * cs[2 * i + 1];
-              if (gamma) {
-                xa[i] *= r;
-                xb[i] *= r;
-                dg[BWD ? key : 0][0][i] += za * xa[i];
-                dg[BWD ? key : 0][1][i] += zb * xb[i];
-                za *= w[0][i];
-                zb *= w[1][i];
-                dot += za * xa[i] + zb * xb[i];
-              }
-              da[i] = za;
-              db[i] = zb;
-            }
-            if (gamma) dot = row_sum<T, HD>(dot) * (1.f / HD);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              ya[i] = gamma ? r * (da[i] - xa[i] * dot) : da[i];
-              yb[i] = gamma ? r * (db[i] - xb[i] * dot) : db[i];
-            }
-          }
-          if (g + u < to && h < heads) {
-            *reinterpret_cast<uint4*>(y + (size_t)h * HD) = pack(ya);
-            *reinterpret_cast<uint4*>(y + (size_t)h * HD + HD / 2) = pack(yb);
+        for (int hf = 0; hf < 2; ++hf) {
+          in[u][hf] = Raw<WORDS>{};
+          if (on && (!BWD || gamma)) load_raw(in[u][hf], x + (size_t)h * HD + hf * (HD / 2));
+          if constexpr (BWD) {
+            up[u][hf] = Raw<WORDS>{};
+            if (on) load_raw(up[u][hf], dy + (size_t)h * HD + hf * (HD / 2));
           }
         }
       }
-    };
-    side(0, a.q, a.ldq, a.dq_out, a.lddqo, a.q_out, a.ldqo, a.q_gamma, a.heads, min(g0, gq), min(g1, gq));
-    side(1, a.k, a.ldk, a.dk_out, a.lddko, a.k_out, a.ldko, a.k_gamma, a.kv_heads, max(g0, gq) - gq, max(g1, gq) - gq);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = (g + u) * V::RPW + sub;
+        float xa[VEC], xb[VEC], ya[VEC], yb[VEC], r = 1.f;
+        unpack<T>(in[u][0], xa);
+        unpack<T>(in[u][1], xb);
+        if (gamma) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) ss += xa[i] * xa[i] + xb[i] * xb[i];
+          r = rsqrtf(row_sum<V::LPR>(ss) * (1.f / HD) + a.eps);
+        }
+        if constexpr (!BWD) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float za = gamma ? xa[i] * r * w[0][i] : xa[i], zb = gamma ? xb[i] * r * w[1][i] : xb[i];
+            ya[i] = za * cs[2 * i] - zb * cs[2 * i + 1];
+            yb[i] = za * cs[2 * i + 1] + zb * cs[2 * i];
+          }
+        } else {
+          float da[VEC], db[VEC], dot = 0.f;
+          unpack<T>(up[u][0], da);
+          unpack<T>(up[u][1], db);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            float za = da[i] * cs[2 * i] + db[i] * cs[2 * i + 1], zb = db[i] * cs[2 * i] - da[i] * cs[2 * i + 1];
+            if (gamma) {
+              xa[i] *= r;
+              xb[i] *= r;
+              dg[0][i] += za * xa[i];
+              dg[1][i] += zb * xb[i];
+              za *= w[0][i];
+              zb *= w[1][i];
+              dot += za * xa[i] + zb * xb[i];
+            }
+            da[i] = za;
+            db[i] = zb;
+          }
+          if (gamma) dot = row_sum<V::LPR>(dot) * (1.f / HD);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            ya[i] = gamma ? r * (da[i] - xa[i] * dot) : da[i];
+            yb[i] = gamma ? r * (db[i] - xb[i] * dot) : db[i];
+          }
+        }
+        if (g + u < g1 && h < heads) {
+          store_raw(y + (size_t)h * HD, pack<T>(ya));
+          store_raw(y + (size_t)h * HD + HD / 2, pack<T>(yb));
+        }
+      }
+    }
   }
   if constexpr (BWD) {
 #pragma unroll
-    for (int key = 0; key < 2; ++key)
+    for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int i = 0; i < VEC; ++i) {
+        float v = dg[hf][i];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float v = dg[key][hf][i];
-#pragma unroll
-          for (int o = 16; o >= V::LPR; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (sub == 0) acc[(warp * 2 + key) * HD + hf * (HD / 2) + at + i] = v;
-        }
+        for (int o = 16; o >= V::LPR; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (sub == 0) acc[warp * HD + hf * (HD / 2) + at + i] = v;
+      }
     write_partial(a, acc);
   }
 }
 
-// Rows that the 16-byte kernel can take.
+// Rows that the vector kernel can take.
 bool vec_ok(const QkNormArgs& a, bool bwd) {
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
   const int es = a.is_bf16 ? 2 : 4;
@@ -382,56 +399,73 @@ bool vec_ok(const QkNormArgs& a, bool bwd) {
   return true;
 }
 
-// A token is one warp's work, or shared by several while tokens alone leave the SMs
-// without kWarpsPerSm warps each.
-constexpr int kWarpsPerSm = 32;
-template <class T, int HD, bool BWD> cudaError_t launch_vec(const QkNormArgs& a, int max_grid, cudaStream_t s, int* grid_out) {
-  using V = VT<T, HD>;
-  const int groups = (a.heads + V::RPW - 1) / V::RPW + (a.kv_heads + V::RPW - 1) / V::RPW;
-  const int64_t want = (int64_t)a.sm_count * kWarpsPerSm;
-  const int slices = (int)std::min<int64_t>(groups, std::max<int64_t>(1, (want + a.tokens - 1) / std::max<int64_t>(1, a.tokens)));
-  const int64_t ctas = (a.tokens * slices + kWarpsPerCta - 1) / kWarpsPerCta;
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(ctas, max_grid));
-  *grid_out = grid;
-  return launch_pdl(qk_norm_vec_kernel<T, HD, BWD>, dim3(grid), dim3(kWarpsPerCta * 32),
-                    BWD ? (size_t)kWarpsPerCta * 2 * HD * sizeof(float) : 0, s, a, slices);
+// CTAs of the queries among `ctas` in proportion to the rows, one at least for each side.
+int queries_part(const QkNormArgs& a, int ctas) {
+  return std::min(ctas - 1, std::max(1, (int)((int64_t)ctas * a.heads / (a.heads + a.kv_heads))));
 }
-template <bool BWD> cudaError_t launch_vec_any(const QkNormArgs& a, int max_grid, cudaStream_t s, int* grid) {
-  switch (a.head_dim) {
-  case 64: return a.is_bf16 ? launch_vec<__nv_bfloat16, 64, BWD>(a, max_grid, s, grid) : launch_vec<float, 64, BWD>(a, max_grid, s, grid);
-  case 128: return a.is_bf16 ? launch_vec<__nv_bfloat16, 128, BWD>(a, max_grid, s, grid) : launch_vec<float, 128, BWD>(a, max_grid, s, grid);
-  default: return a.is_bf16 ? launch_vec<__nv_bfloat16, 256, BWD>(a, max_grid, s, grid) : launch_vec<float, 256, BWD>(a, max_grid, s, grid);
+
+// A token's side is one warp's work, or shared by several while tokens alone leave the
+// SMs without kWarpsPerSm warps each.
+constexpr int kWarpsPerSm = 32;
+template <class T, int HD, bool BWD> cudaError_t launch_vec(const QkNormArgs& a, cudaStream_t s, int* parts, int* part_q) {
+  using V = VT<T, HD, BWD>;
+  const int gq = (a.heads + V::RPW - 1) / V::RPW, gk = (a.kv_heads + V::RPW - 1) / V::RPW;
+  const int64_t tokens = std::max<int64_t>(1, a.tokens);
+  const int64_t want = ((int64_t)a.sm_count * kWarpsPerSm + tokens - 1) / tokens;  // warps a token
+  const auto share = [&](int g) { return (int)std::max<int64_t>(1, std::min<int64_t>(g, (want * g + gq + gk - 1) / (gq + gk))); };
+  const int sq = share(gq), sk = share(gk);
+  const auto ctas = [&](int heads, int slices) { return heads ? (tokens * slices + kWarpsPerCta - 1) / kWarpsPerCta : 1; };
+  int64_t cq = ctas(a.heads, sq), ck = ctas(a.kv_heads, sk);
+  if (cq + ck > kQkNormParts && BWD) {  // a partial row of the gamma gradients for each CTA
+    cq = queries_part(a, kQkNormParts);
+    ck = kQkNormParts - cq;
   }
+  *part_q = (int)cq;
+  *parts = (int)(cq + ck);
+  return launch_pdl(qk_norm_vec_kernel<T, HD, BWD>, dim3((unsigned)*parts), dim3(kWarpsPerCta * 32),
+                    BWD ? (size_t)kWarpsPerCta * HD * sizeof(float) : 0, s, a, *part_q, sq, sk);
+}
+template <bool BWD> cudaError_t launch_vec_any(const QkNormArgs& a, cudaStream_t s, int* parts, int* part_q) {
+  const auto go = [&](auto t) {
+    using T = decltype(t);
+    switch (a.head_dim) {
+    case 64: return launch_vec<T, 64, BWD>(a, s, parts, part_q);
+    case 128: return launch_vec<T, 128, BWD>(a, s, parts, part_q);
+    default: return launch_vec<T, 256, BWD>(a, s, parts, part_q);
+    }
+  };
+  return a.is_bf16 ? go(__nv_bfloat16{}) : go(float{});
 }
 
 }  // namespace
 
-size_t qk_norm_workspace_bytes(int head_dim) { return (size_t)kQkNormParts * 2 * head_dim * sizeof(float); }
+size_t qk_norm_workspace_bytes(int head_dim) { return (size_t)kQkNormParts * head_dim * sizeof(float); }
 
 cudaError_t qk_norm_forward(const QkNormArgs& a, cudaStream_t s) {
   const int64_t rows = a.tokens * (a.heads + a.kv_heads);
   if (rows == 0) return cudaSuccess;
-  int grid = 0;
-  if (vec_ok(a, false)) return launch_vec_any<false>(a, 1 << 30, s, &grid);
-  grid = (int)std::min<int64_t>((rows + kWarpsPerCta - 1) / kWarpsPerCta, (int64_t)a.sm_count * 64);
+  int parts = 0, part_q = 0;
+  if (vec_ok(a, false)) return launch_vec_any<false>(a, s, &parts, &part_q);
+  const int grid = (int)std::min<int64_t>((rows + kWarpsPerCta - 1) / kWarpsPerCta, (int64_t)a.sm_count * 64);
   return a.is_bf16 ? launch_pdl(qk_norm_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(kWarpsPerCta * 32), 0, s, a)
                    : launch_pdl(qk_norm_rows_kernel<float>, dim3(grid), dim3(kWarpsPerCta * 32), 0, s, a);
 }
 
 cudaError_t qk_norm_backward(const QkNormArgs& a, cudaStream_t s) {
   const int64_t rows = a.tokens * (a.heads + a.kv_heads);
-  int parts = 0;
+  int parts = 0, part_q = 0;
   cudaError_t e;
   if (vec_ok(a, true)) {
-    e = launch_vec_any<true>(a, kQkNormParts, s, &parts);
+    e = launch_vec_any<true>(a, s, &parts, &part_q);
   } else {
-    parts = (int)std::max<int64_t>(1, std::min<int64_t>((rows + kWarpsPerCta - 1) / kWarpsPerCta, kQkNormParts));
-    const size_t smem = (size_t)kWarpsPerCta * 2 * a.head_dim * sizeof(float);
-    e = a.is_bf16 ? launch_pdl(qk_norm_rows_bwd_kernel<__nv_bfloat16>, dim3(parts), dim3(kWarpsPerCta * 32), smem, s, a)
-                  : launch_pdl(qk_norm_rows_bwd_kernel<float>, dim3(parts), dim3(kWarpsPerCta * 32), smem, s, a);
+    parts = (int)std::max<int64_t>(2, std::min<int64_t>((rows + kWarpsPerCta - 1) / kWarpsPerCta, kQkNormParts));
+    part_q = queries_part(a, parts);
+    const size_t smem = (size_t)kWarpsPerCta * a.head_dim * sizeof(float);
+    e = a.is_bf16 ? launch_pdl(qk_norm_rows_bwd_kernel<__nv_bfloat16>, dim3(parts), dim3(kWarpsPerCta * 32), smem, s, a, part_q)
+                  : launch_pdl(qk_norm_rows_bwd_kernel<float>, dim3(parts), dim3(kWarpsPerCta * 32), smem, s, a, part_q);
   }
   if (e != cudaSuccess || (!a.dq_gamma && !a.dk_gamma)) return e;
-  return launch_pdl(dgamma_kernel, dim3((2 * a.head_dim + 31) / 32), dim3(1024), 0, s, (const float*)a.partial, parts,
+  return launch_pdl(dgamma_kernel, dim3((a.head_dim + 31) / 32, 2), dim3(1024), 0, s, (const float*)a.partial, part_q, parts,
                     a.head_dim, a.dq_gamma, a.dk_gamma);
 }
 

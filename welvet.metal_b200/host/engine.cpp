@@ -170,11 +170,13 @@ const char* err_reason(uint32_t code) {
 } // namespace
 
 Status device_ctx(int device, DeviceCtx** out) {
-  if (device < 0) WV_CUDA(cudaGetDevice(&device), "cudaGetDevice");
+  const bool current = device < 0;
+  if (current) WV_CUDA(cudaGetDevice(&device), "cudaGetDevice");
   std::lock_guard<std::mutex> lock(g_dev_mu);
   auto it = g_devs.find(device);
   if (it != g_devs.end()) {
     *out = it->second;
+    if (current) return Status::ok();  // its context exists, and it is current already
     return cudaSetDevice(device) == cudaSuccess ? Status::ok() : Status::err(4, "cudaSetDevice");
   }
   WV_CUDA(cudaSetDevice(device), "cudaSetDevice");

@@ -227,23 +227,22 @@ def _ptr(a):
 _DTYPE_NAMES: dict = {}
 
 
-def _dtype_name(t) -> str:
-    """"bfloat16" for a tensor of torch.bfloat16 and so on, without importing torch."""
-    name = _DTYPE_NAMES.get(t.dtype)
+def _dtype_name(dtype) -> str:
+    """"bfloat16" for torch.bfloat16 and so on, without importing torch."""
+    name = _DTYPE_NAMES.get(dtype)
     if name is None:
-        name = _DTYPE_NAMES[t.dtype] = str(t.dtype).replace("torch.", "")
+        name = _DTYPE_NAMES[dtype] = str(dtype).replace("torch.", "")
     return name
 
 
-def _rows(t, width):
-    """(pointer, row stride) of a 2-D device tensor of at least `width` values a row, the
-    values of a row next to each other; (None, width) for None."""
-    if t is None:
-        return None, width
-    (rows, cols), (ld, step) = t.shape, t.stride()
-    if cols < width or (step != 1 and cols > 1):
-        raise ValueError(f"rows of at least {width} adjacent values expected, got {tuple(t.shape)}")
-    return t.data_ptr(), (ld if rows > 1 else max(ld, cols))
+def _rows(t, rows, width, dtype):
+    """(pointer, row stride) of a 2-D device tensor of `dtype` with at least `rows` rows of
+    `width` values, the values of a row next to each other."""
+    n, cols = t.shape
+    ld, step = t.stride()
+    if n < rows or cols < width or t.dtype != dtype or (step != 1 and cols > 1):
+        raise ValueError(f"{rows} rows of {width} adjacent {dtype} values expected, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr(), (ld if n > 1 else max(ld, cols))
 
 
 def _stream(s):
@@ -545,27 +544,27 @@ def _typed(t, dtype, numel=0):
     """Device pointer of a contiguous tensor of the given dtype and at least numel values."""
     if t is None:
         return None
-    if _dtype_name(t) != dtype or t.numel() < numel or not t.is_contiguous():
+    if (_DTYPE_NAMES.get(t.dtype) or _dtype_name(t.dtype)) != dtype or t.numel() < numel or not t.is_contiguous():
         raise ValueError(f"contiguous {dtype} of at least {numel} values expected, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _norm_call(q, k, others, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod):
-    """(io_bf16, the leading arguments, row widths) of a norm call; `others` have the
-    tokens and the dtype of q."""
+def _norm_call(q, k, pairs, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod):
+    """(io_bf16, arguments) of a norm call up to the row pointers; `pairs` are (queries,
+    keys) tensors with the tokens, widths and dtype of q and k."""
     tokens, qd = q.shape
     kd = 0 if k is None else k.shape[1]
-    for t in (k, *others):
-        if t is not None and (t.shape[0] != tokens or t.dtype != q.dtype):
-            raise ValueError("q, k, their outputs and gradients need the same tokens and dtype")
-    io = {"bfloat16": 1, "float32": 0}.get(_dtype_name(q))
-    if io is None or qd % head_dim or kd % head_dim:
+    dtype = q.dtype
+    io = 1 if _dtype_name(dtype) == "bfloat16" else 0
+    if (not io and _dtype_name(dtype) != "float32") or head_dim <= 0 or qd % head_dim or kd % head_dim:
         raise ValueError("BF16 or FP32 rows of whole heads expected")
-    args = (tokens, qd // head_dim, kd // head_dim, head_dim, eps, _typed(q_gamma, "float32", head_dim),
+    args = [tokens, qd // head_dim, kd // head_dim, head_dim, eps, _typed(q_gamma, "float32", head_dim),
             _typed(k_gamma, "float32", head_dim), _typed(rope, "float32"),
-            0 if rope is None else rope.numel() // head_dim, _typed(positions, "int32", tokens), pos_mod,
-            *_rows(q, qd), *_rows(k, kd))
-    return io, args, qd, kd
+            0 if rope is None else rope.numel() // head_dim, _typed(positions, "int32", tokens), pos_mod]
+    for a, b in ((q, k),) + pairs:
+        args += _rows(a, tokens, qd, dtype)
+        args += _rows(b, tokens, kd, dtype) if kd else (None, 0)
+    return io, args
 
 
 def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1e-6, rope=None, positions=None,
@@ -573,8 +572,8 @@ def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1
     """RMS norm of every query and key head with the rotation in the same pass
     (welvet_b200_qk_norm_rope_forward): rows [tokens, heads * head_dim] (may be views of
     one packed row; k may be None), outputs may be the inputs."""
-    io, args, qd, kd = _norm_call(q, k, (q_out, k_out), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
-    check(lib().welvet_b200_qk_norm_rope_forward(*args, *_rows(q_out, qd), *_rows(k_out, kd), io, _stream(stream)))
+    io, args = _norm_call(q, k, ((q_out, k_out),), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    check(lib().welvet_b200_qk_norm_rope_forward(*args, io, _stream(stream)))
 
 
 def qk_norm_rope_workspace(head_dim) -> int:
@@ -587,14 +586,12 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, dq_gamma, dk_gamma, head
     """Gradient of qk_norm_rope (welvet_b200_qk_norm_rope_backward): dq, dk from the
     forward's inputs and the gradients of its outputs, dq_gamma / dk_gamma [head_dim]
     overwritten with the sums over all rows."""
-    io, args, qd, kd = _norm_call(q, k, (dq_out, dk_out, dq, dk), head_dim, q_gamma, k_gamma, eps, rope, positions,
-                                  pos_mod)
+    io, args = _norm_call(q, k, ((dq_out, dk_out), (dq, dk)), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
     if workspace.numel() * workspace.element_size() < qk_norm_rope_workspace(head_dim):
         raise ValueError("workspace smaller than qk_norm_rope_workspace(head_dim)")
-    check(lib().welvet_b200_qk_norm_rope_backward(
-        *args, *_rows(dq_out, qd), *_rows(dk_out, kd), *_rows(dq, qd), *_rows(dk, kd),
-        _typed(dq_gamma, "float32", head_dim), _typed(dk_gamma, "float32", head_dim), _ptr(workspace), io,
-        _stream(stream)))
+    check(lib().welvet_b200_qk_norm_rope_backward(*args, _typed(dq_gamma, "float32", head_dim),
+                                                  _typed(dk_gamma, "float32", head_dim), _ptr(workspace), io,
+                                                  _stream(stream)))
 
 
 class Kv8Cache:
@@ -611,36 +608,37 @@ class Kv8Cache:
         batch, max_pages = block_table.shape
         n = pages * kv_heads * (self.PAGE // self.BLOCK)
         self.tensors = (k, v, k_scale, v_scale, block_table, ctx_len)
+        self.batch, self.head_dim, self.width = batch, head_dim, kv_heads * head_dim
         self.args = _Kv8CacheArgs(_ptr(k), _ptr(v), _typed(k_scale, "float32", n),
                                   _typed(v_scale, "float32", n), _typed(block_table, "int32"),
                                   _typed(ctx_len, "int32", batch), batch, pages, max_pages, kv_heads, head_dim)
+        self.ref = C.byref(self.args)
 
 
-def _bf16_rows(t, rows, width):
-    if _dtype_name(t) != "bfloat16" or t.shape[0] < rows:
-        raise ValueError(f"{rows} BF16 rows expected, got {t.dtype} {tuple(t.shape)}")
-    return _rows(t, width)
+def _bf16(t):
+    dtype = t.dtype
+    if _dtype_name(dtype) != "bfloat16":
+        raise ValueError(f"BF16 rows expected, got {dtype}")
+    return dtype
 
 
 def kv8_append(cache: Kv8Cache, seq, k, v, rope=None, seq_lens=None, stream=None):
     """Appends rows b * seq + t of k and v (BF16 [batch * seq, kv_heads * head_dim], may be
     views of packed rows) to the cache (welvet_b200_kv8_append)."""
-    c = cache.args
-    width = c.kv_heads * c.head_dim
-    check(lib().welvet_b200_kv8_append(C.byref(c), seq, _typed(seq_lens, "int32", c.batch),
-                                       *_bf16_rows(k, c.batch * seq, width), *_bf16_rows(v, c.batch * seq, width),
-                                       _typed(rope, "float32"), 0 if rope is None else rope.numel() // c.head_dim,
+    dtype, rows, width = _bf16(k), cache.batch * seq, cache.width
+    check(lib().welvet_b200_kv8_append(cache.ref, seq, _typed(seq_lens, "int32", cache.batch),
+                                       *_rows(k, rows, width, dtype), *_rows(v, rows, width, dtype),
+                                       _typed(rope, "float32"), 0 if rope is None else rope.numel() // cache.head_dim,
                                        _stream(stream)))
 
 
 def kv8_attention(cfg: MhaConfig, cache: Kv8Cache, seq, q, out, max_ctx, seq_lens=None, stream=None):
     """Attention of the new tokens (BF16 rows b * seq + t of q) over the cache
     (welvet_b200_kv8_attention)."""
-    c = cache.args
-    width = (cfg.head_count if cfg.head_count > 0 else cfg.num_heads) * c.head_dim
-    check(lib().welvet_b200_kv8_attention(C.byref(cfg), C.byref(c), seq, _typed(seq_lens, "int32", c.batch),
-                                          max_ctx, *_bf16_rows(q, c.batch * seq, width),
-                                          *_bf16_rows(out, c.batch * seq, width), _stream(stream)))
+    dtype, rows, width = _bf16(q), cache.batch * seq, (cfg.head_count or cfg.num_heads) * cache.head_dim
+    check(lib().welvet_b200_kv8_attention(C.byref(cfg), cache.ref, seq, _typed(seq_lens, "int32", cache.batch), max_ctx,
+                                          *_rows(q, rows, width, dtype), *_rows(out, rows, width, dtype),
+                                          _stream(stream)))
 
 
 def codec_roundtrip(dtype, w, out, stream=None):
