@@ -130,6 +130,28 @@ WELVET_API welvet_status welvet_b200_mha_decode(welvet_b200_mha* layer, welvet_b
                                                 int32_t batch, const void* x_new, void* pre,
                                                 void* post, int32_t on_device, void* stream);
 
+/* The same cache in E4M3: half the bytes of BF16, in pages of 64 tokens with a
+ * power-of-two scale for each 16 tokens of a KV head (welvet_b200_kv8_append below
+ * states the rule). kv_fill, mha_prefill, mha_decode and mha_extend take it in place of
+ * the other. Layers with BF16 activations, softmax scores, a causal or causal-window
+ * mask and an even head_dim of at most 256; otherwise code 2. */
+WELVET_API welvet_status welvet_b200_kv_create_e4m3(welvet_b200_mha* layer, int32_t max_batch,
+                                                    int32_t max_ctx, welvet_b200_kv** out);
+/* seq new tokens per sequence at positions ctx_len[b] ... ctx_len[b] + seq - 1 (a later
+ * piece of a prompt, proposed tokens to verify): x_new, post [batch * seq, d_model], row
+ * b * seq + t; their keys and values are appended and every row attends over the cache up
+ * to its own position. E4M3 caches (code 2 otherwise); seq 1 is mha_decode. */
+WELVET_API welvet_status welvet_b200_mha_extend(welvet_b200_mha* layer, welvet_b200_kv* kv,
+                                                int32_t batch, int32_t seq, const void* x_new, void* pre,
+                                                void* post, int32_t on_device, void* stream);
+/* RMS norm of every query and key head between the projection and the position encoding
+ * (welvet_b200_qk_norm_rope_forward below), in every forward, prefill, decode and extend
+ * of the layer from now on; q_gamma, k_gamma [head_dim] FP32 are copied (host or device
+ * per on_device; synchronises). Both NULL: no norm. eps <= 0 selects 1e-6. */
+WELVET_API welvet_status welvet_b200_mha_set_qk_norm(welvet_b200_mha* layer, double eps,
+                                                     const float* q_gamma, const float* k_gamma,
+                                                     int32_t on_device);
+
 /* ---- multi-GPU (no reference counterpart: the reference is single-device) ----
  * One process per GPU. Rank 0 creates the id, the caller distributes it; every
  * rank attaches an NCCL communicator to its head-sharded layer. */
@@ -271,8 +293,9 @@ WELVET_API welvet_status welvet_b200_decode_attention_static(const welvet_b200_m
 /* ---- q/k norms and the E4M3 KV cache (no counterpart in the reference) ----
  * Device buffers, asynchronous on `stream`; nothing is allocated after the first
  * call on a device. Code 1 for invalid arguments, 2 for what is not built. Device
- * faults of the data (a position past the RoPE table, a page outside the pool) leave
- * the row or block out and are reported by welvet_b200_device_check.
+ * faults of the data are reported by welvet_b200_device_check and touch nothing out of
+ * range: a position past the RoPE table leaves its row unrotated, a page outside the
+ * pool its block unwritten and the attention rows that needed it unspecified.
  *
  * RoPE table: (cos, sin) of pos / theta^(2i/head_dim), [max_pos][head_dim/2][2] FP32,
  * computed in FP64, the table the layer uses (shaders/ops_mha.metal:14-29). */

@@ -193,10 +193,28 @@ welvet_status welvet_b200_kv_create(welvet_b200_mha* layer, int32_t max_batch, i
   wv::DeviceRestore restore_device;
   if (!layer || !out) return wv::to_c(Status::err(1, "kv: invalid argument"));
   wv::Kv* kv = nullptr;
-  Status st = wv::kv_create(layer->m, max_batch, max_ctx, &kv);
+  Status st = wv::kv_create(layer->m, max_batch, max_ctx, false, &kv);
   if (!st) return wv::to_c(st);
   *out = new welvet_b200_kv{kv};
   return ok_status();
+}
+
+welvet_status welvet_b200_kv_create_e4m3(welvet_b200_mha* layer, int32_t max_batch, int32_t max_ctx,
+                                         welvet_b200_kv** out) {
+  wv::DeviceRestore restore_device;
+  if (!layer || !out) return wv::to_c(Status::err(1, "kv: invalid argument"));
+  wv::Kv* kv = nullptr;
+  Status st = wv::kv_create(layer->m, max_batch, max_ctx, true, &kv);
+  if (!st) return wv::to_c(st);
+  *out = new welvet_b200_kv{kv};
+  return ok_status();
+}
+
+welvet_status welvet_b200_mha_set_qk_norm(welvet_b200_mha* layer, double eps, const float* q_gamma,
+                                          const float* k_gamma, int32_t on_device) {
+  wv::DeviceRestore restore_device;
+  if (!layer) return wv::to_c(Status::err(1, "mha qk_norm: nil layer"));
+  return wv::to_c(wv::mha_set_qk_norm(layer->m, eps, q_gamma, k_gamma, on_device != 0));
 }
 
 void welvet_b200_kv_release(welvet_b200_kv* kv) {
@@ -228,7 +246,14 @@ welvet_status welvet_b200_mha_decode(welvet_b200_mha* layer, welvet_b200_kv* kv,
                                      void* pre, void* post, int32_t on_device, void* stream) {
   wv::DeviceRestore restore_device;
   if (!layer || !kv) return wv::to_c(Status::err(1, "mha decode: invalid argument"));
-  return wv::to_c(wv::mha_decode(layer->m, kv->kv, batch, x_new, pre, post, on_device != 0, as_stream(stream)));
+  return wv::to_c(wv::mha_decode(layer->m, kv->kv, batch, 1, x_new, pre, post, on_device != 0, as_stream(stream)));
+}
+
+welvet_status welvet_b200_mha_extend(welvet_b200_mha* layer, welvet_b200_kv* kv, int32_t batch, int32_t seq,
+                                     const void* x_new, void* pre, void* post, int32_t on_device, void* stream) {
+  wv::DeviceRestore restore_device;
+  if (!layer || !kv) return wv::to_c(Status::err(1, "mha extend: invalid argument"));
+  return wv::to_c(wv::mha_decode(layer->m, kv->kv, batch, seq, x_new, pre, post, on_device != 0, as_stream(stream)));
 }
 
 welvet_status welvet_b200_comm_unique_id(uint8_t id[128]) { return wv::to_c(wv::comm_unique_id(id)); }

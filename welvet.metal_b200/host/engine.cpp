@@ -462,6 +462,39 @@ Status ensure_io_streams(Mha* m) {
   return Status::ok();
 }
 
+// The cache as kernel arguments (E4M3 caches).
+Kv8Cache kv8_args(const Kv* kv) {
+  Kv8Cache c;
+  c.k = kv->k_pool.p;
+  c.v = kv->v_pool.p;
+  c.k_scale = kv->k_scale.as<float>();
+  c.v_scale = kv->v_scale.as<float>();
+  c.block_table = kv->block_table.as<int>();
+  c.ctx_len = kv->ctx_len.as<int>();
+  c.pages = kv->max_batch * kv->pages_per_seq;
+  c.max_pages = kv->pages_per_seq;
+  c.kv_heads = kv->layer->khc;
+  c.head_dim = kv->layer->cfg.hd;
+  return c;
+}
+
+// The last seq tokens of every sequence (positions ctx_len - seq ...) into the cache, from
+// rows ld apart, position encoding done.
+Status kv8_append_rows(Kv* kv, int batch, int seq, const void* k, const void* v, int ld, cudaStream_t s) {
+  Kv8AppendArgs a;
+  a.c = kv8_args(kv);
+  a.batch = batch;
+  a.seq = seq;
+  a.k = k;
+  a.v = v;
+  a.ldk = a.ldv = ld;
+  a.err = kv->layer->dev->err;
+  a.sm_count = kv->layer->dev->sm_count;
+  WV_CUDA(kv8_append(a, s), "kv8 append");
+  count_launch();
+  return Status::ok();
+}
+
 Status ensure_rope(Mha* m, int max_pos, cudaStream_t s) {
   if (!m->cfg.rope || m->cfg.hd < 2) return Status::ok();
   if (max_pos <= m->rope_max_pos) return Status::ok();
@@ -553,7 +586,8 @@ Status run_proj(Mha* m, const Proj& pj, cudaStream_t s, bool* kv_done = nullptr)
   g.err = m->dev->err;
   g.split_only = pj.split_only ? 1 : 0;
   g.sm_count = m->dev->sm_count;
-  const bool rope = pj.rope_cols > 0 && m->cfg.rope;
+  const bool norm = pj.rope_cols > 0 && m->qk_norm;  // rotates too, in place of the fused rotation
+  const bool rope = pj.rope_cols > 0 && m->cfg.rope && !norm;
   if (rope) {
     g.rope_tab = m->rope_tab.as<float2>();
     g.rope_cols = pj.rope_cols;
@@ -563,10 +597,37 @@ Status run_proj(Mha* m, const Proj& pj, cudaStream_t s, bool* kv_done = nullptr)
     g.pos_mod = pj.pos_mod;
   }
   const int hd = m->cfg.hd;
+  const auto norm_rows = [&]() -> Status {
+    QkNormArgs a;
+    a.tokens = pj.M;
+    a.heads = m->hc;
+    a.kv_heads = m->khc;
+    a.head_dim = hd;
+    a.is_bf16 = f32 ? 0 : 1;
+    a.eps = m->qk_eps;
+    a.q_gamma = m->qk_gamma.as<float>();
+    a.k_gamma = a.q_gamma + hd;
+    a.rope = m->cfg.rope ? m->rope_tab.as<float2>() : nullptr;
+    a.max_pos = m->rope_max_pos;
+    a.positions = pj.positions;
+    a.pos_mod = pj.pos_mod;
+    a.q = a.q_out = pj.out;
+    a.k = a.k_out = static_cast<char*>(pj.out) + (size_t)m->qd_l * (f32 ? 4 : 2);
+    a.ldq = a.ldk = a.ldqo = a.ldko = pj.ldo;
+    a.err = m->dev->err;
+    a.sm_count = m->dev->sm_count;
+    WV_CUDA(qk_norm_forward(a, s), "qk norm");
+    count_launch();
+    if (pj.out_hi) {  // keep the TF32 split in step
+      WV_CUDA(split_tf32(static_cast<const float*>(pj.out), pj.out_hi, pj.out_lo, (int64_t)pj.M * pj.ldo, s), "split");
+      count_launch();
+    }
+    return Status::ok();
+  };
   if (pj.splitk && !f32 && decode_gemv_enabled()) {
     GemmArgs v = g;
     v.head_dim = hd;
-    v.kv_k = pj.kv_k;
+    v.kv_k = norm ? nullptr : pj.kv_k;  // the kernel's keys are not the cache's yet
     v.kv_v = pj.kv_v;
     v.kv_slot = pj.kv_slot;
     v.kv_col0 = pj.kv_col0;
@@ -574,13 +635,13 @@ Status run_proj(Mha* m, const Proj& pj, cudaStream_t s, bool* kv_done = nullptr)
     if (gemv_decode_supported(v)) {
       WV_CUDA(gemv_decode(v, s), "gemv_decode");
       count_launch();
-      if (kv_done) *kv_done = pj.kv_k != nullptr;
-      return Status::ok();
+      if (kv_done) *kv_done = v.kv_k != nullptr;
+      return norm ? norm_rows() : Status::ok();
     }
   }
   const int bn = f32 ? 128 : 256;
   const bool fused_rope = rope && (hd == 64 || hd == 128 || hd == 256) && bn % hd == 0;
-  if (rope && !fused_rope) g.split_only = 0;  // rope_apply rotates out, then re-splits it
+  if ((rope && !fused_rope) || norm) g.split_only = 0;  // out is rotated, then split again
   if (gemm_tc_supported(g)) {
     if (pj.splitk) {
       const size_t floats = gemm_tc_splitk_floats(g);
@@ -608,7 +669,7 @@ Status run_proj(Mha* m, const Proj& pj, cudaStream_t s, bool* kv_done = nullptr)
       count_launch();
     }
   }
-  return Status::ok();
+  return norm ? norm_rows() : Status::ok();
 }
 
 AttnArgs attn_args(Mha* m, int batch, int seq, bool stream_mode) {
@@ -798,7 +859,14 @@ Status mha_forward(Mha* m, int batch, int seq, const void* x, void* pre, void* p
     WV_TRY(run_proj(m, q, s));
     prof_end(kProfGemmQkv, s);
 
-    if (kv) {  // prefill: K/V rows into the cache pages of each sequence (single chunk)
+    if (kv && kv->e4m3) {  // prefill into an E4M3 cache (single chunk)
+      WV_CUDA(set_ctx(kv->ctx_len.as<int>(), batch, seq, s), "ctx");
+      count_launch();
+      const char* base = static_cast<const char*>(m->qkv.p);
+      WV_TRY(kv8_append_rows(kv, batch, seq, base + (size_t)m->qd_l * es, base + (size_t)(m->qd_l + m->kd_l) * es,
+                             m->nqkv, s));
+      for (int b = 0; b < batch; ++b) kv->ctx_host[b] = seq;
+    } else if (kv) {  // prefill: K/V rows into the cache pages of each sequence (single chunk)
       WV_TRY(m->slots.ensure(M * 4));
       WV_CUDA(make_prefill_slots(m->slots.as<int>(), batch, seq, kv->pages_per_seq, s), "slots");
       const char* base = static_cast<const char*>(m->qkv.p);
@@ -1090,16 +1158,49 @@ Status mha_forward(Mha* m, int batch, int seq, const void* x, void* pre, void* p
 }
 
 // ------------------------------------------------------------------ KV cache
-Status kv_create(Mha* m, int max_batch, int max_ctx, Kv** out) {
+Status mha_set_qk_norm(Mha* m, double eps, const float* q_gamma, const float* k_gamma, bool on_device) {
+  if (!m || (q_gamma == nullptr) != (k_gamma == nullptr) || std::isnan(eps))
+    return Status::err(1, "mha qk_norm: invalid argument");
+  std::lock_guard<std::mutex> lock(m->mu);
+  if (!q_gamma) {
+    m->qk_norm = false;
+    return Status::ok();
+  }
+  const int hd = m->cfg.hd;
+  if (hd % 2 || hd > kQkNormMaxHeadDim)
+    return Status::err(2, "mha qk_norm: head_dim must be even and at most " + std::to_string(kQkNormMaxHeadDim));
+  WV_CUDA(cudaSetDevice(m->dev->device), "cudaSetDevice");
+  WV_CUDA(cudaDeviceSynchronize(), "qk norm");  // a forward on another stream may still read the old ones
+  WV_TRY(m->qk_gamma.ensure((size_t)2 * hd * 4));
+  const cudaMemcpyKind kind = on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice;
+  WV_CUDA(cudaMemcpy(m->qk_gamma.p, q_gamma, (size_t)hd * 4, kind), "qk norm gamma");
+  WV_CUDA(cudaMemcpy(m->qk_gamma.as<float>() + hd, k_gamma, (size_t)hd * 4, kind), "qk norm gamma");
+  WV_CUDA(cudaDeviceSynchronize(), "qk norm");
+  m->qk_eps = eps > 0 ? (float)eps : 1e-6f;
+  m->qk_norm = true;
+  return Status::ok();
+}
+
+Status kv_create(Mha* m, int max_batch, int max_ctx, bool e4m3, Kv** out) {
   if (!m || max_batch <= 0 || max_ctx <= 0 || !out) return Status::err(1, "kv: invalid argument");
+  if (e4m3) WV_TRY(kv8_supported(m->cfg, "kv"));
   WV_CUDA(cudaSetDevice(m->dev->device), "cudaSetDevice");
   auto kv = std::make_unique<Kv>();
   kv->layer = m;
   kv->max_batch = max_batch;
   kv->max_ctx = max_ctx;
-  kv->pages_per_seq = (max_ctx + kPageTokens - 1) / kPageTokens;
-  const size_t es = m->precision == 0 ? 4 : 2;
-  const size_t pool = (size_t)max_batch * kv->pages_per_seq * kPageTokens * m->kd_l * es;
+  kv->e4m3 = e4m3;
+  const int page = e4m3 ? kKv8Page : kPageTokens;
+  kv->pages_per_seq = (max_ctx + page - 1) / page;
+  if (e4m3 && (max_batch > 65535 || (int64_t)max_batch * kv->pages_per_seq > INT32_MAX))
+    return Status::err(1, "kv: max_batch or max_ctx too large");
+  const size_t es = e4m3 ? 1 : m->precision == 0 ? 4 : 2;
+  const size_t pool = (size_t)max_batch * kv->pages_per_seq * page * m->kd_l * es;
+  if (e4m3) {
+    const size_t scales = (size_t)max_batch * kv->pages_per_seq * m->khc * kKv8Subs * 4;
+    WV_TRY(kv->k_scale.ensure(scales));
+    WV_TRY(kv->v_scale.ensure(scales));
+  }
   WV_TRY(kv->k_pool.ensure(pool));
   WV_TRY(kv->v_pool.ensure(pool));
   WV_TRY(kv->block_table.ensure((size_t)max_batch * kv->pages_per_seq * 4));
@@ -1133,6 +1234,14 @@ Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on
       kd = tk.p;
       vd = tv.p;
     }
+    if (kv->e4m3) {
+      WV_CUDA(set_ctx(kv->ctx_len.as<int>(), batch, ctx, s), "ctx");
+      count_launch();
+      WV_TRY(kv8_append_rows(kv, batch, ctx, kd, vd, m->kd_l, s));
+      for (int b = 0; b < batch; ++b) kv->ctx_host[b] = ctx;
+      if (!on_device) WV_CUDA(cudaStreamSynchronize(s), "kv fill");
+      return Status::ok();
+    }
     WV_TRY(m->slots.ensure(rows * 4));
     WV_CUDA(make_prefill_slots(m->slots.as<int>(), batch, ctx, kv->pages_per_seq, s), "slots");
     WV_CUDA(kv_append(kd, vd, m->kd_l, (int)rows, m->kd_l, m->cfg.hd, m->precision == 1, m->slots.as<int>(),
@@ -1147,10 +1256,14 @@ Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on
   return Status::ok();
 }
 
-Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* post, bool on_device,
+Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, void* post, bool on_device,
                   cudaStream_t s) {
-  if (!m || !kv || kv->layer != m || !x || !post || batch <= 0 || batch > kv->max_batch)
+  if (!m || !kv || kv->layer != m || !x || !post || batch <= 0 || batch > kv->max_batch || seq <= 0 ||
+      (int64_t)batch * seq >= (int64_t{1} << 30))
     return Status::err(1, "mha decode: invalid argument");
+  if (seq > 1 && !kv->e4m3) return Status::err(2, "mha extend: needs an E4M3 cache");
+  if ((int64_t)seq * m->hc > INT32_MAX) return Status::err(1, "mha extend: seq * heads too large");
+  const int rows = batch * seq;
   std::lock_guard<std::mutex> lock(m->mu);
   WV_CUDA(cudaSetDevice(m->dev->device), "cudaSetDevice");
   const auto& c = m->cfg;
@@ -1159,28 +1272,32 @@ Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* pos
   const size_t es = f32 ? 4 : 2;
   int max_ctx = 0;
   for (int b = 0; b < batch; ++b) max_ctx = std::max(max_ctx, kv->ctx_host[b]);
-  if (max_ctx + 1 > kv->max_ctx) return Status::err(1, "mha decode: KV cache full");
-  WV_TRY(ensure_rope(m, max_ctx + 1, s));
+  if ((int64_t)max_ctx + seq > kv->max_ctx) return Status::err(1, "mha decode: KV cache full");
+  WV_TRY(ensure_rope(m, max_ctx + seq, s));
 
   const void* xd = x;
   void* postd = post;
   if (!on_device) {
-    WV_TRY(m->x_io.ensure((size_t)batch * dm * es));
-    WV_TRY(m->post_io.ensure((size_t)batch * dm * es));
-    WV_CUDA(cudaMemcpyAsync(m->x_io.p, x, (size_t)batch * dm * es, cudaMemcpyHostToDevice, s), "H2D x");
+    WV_TRY(m->x_io.ensure((size_t)rows * dm * es));
+    WV_TRY(m->post_io.ensure((size_t)rows * dm * es));
+    WV_CUDA(cudaMemcpyAsync(m->x_io.p, x, (size_t)rows * dm * es, cudaMemcpyHostToDevice, s), "H2D x");
     xd = m->x_io.p;
     postd = m->post_io.p;
   }
-  WV_TRY(m->positions.ensure((size_t)batch * 4));
+  WV_TRY(m->positions.ensure((size_t)rows * 4));
   WV_TRY(m->slots.ensure((size_t)batch * 4));
-  // positions[b] = ctx[b]; slots[b] = page slot of that position; ctx[b] += 1
-  WV_CUDA(make_decode_rows(kv->ctx_len.as<int>(), m->positions.as<int>(), m->slots.as<int>(), batch,
-                           kv->pages_per_seq, s), "decode rows");
+  if (kv->e4m3) {
+    WV_CUDA(make_extend_rows(kv->ctx_len.as<int>(), m->positions.as<int>(), batch, seq, s), "decode rows");
+  } else {
+    // positions[b] = ctx[b]; slots[b] = page slot of that position; ctx[b] += 1
+    WV_CUDA(make_decode_rows(kv->ctx_len.as<int>(), m->positions.as<int>(), m->slots.as<int>(), batch,
+                             kv->pages_per_seq, s), "decode rows");
+  }
   count_launch();
-  WV_TRY(m->qkv.ensure((size_t)batch * m->nqkv * es));
+  WV_TRY(m->qkv.ensure((size_t)rows * m->nqkv * es));
 
   Proj q;
-  q.M = batch;
+  q.M = rows;
   q.K = dm;
   q.lda = dm;
   q.N = m->nqkv;
@@ -1193,18 +1310,18 @@ Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* pos
   q.w_lo = m->wqkv_lo.p;
   q.w_scale = m->wqkv_scale.as<float>();
   if (f32) {
-    WV_TRY(m->x_hi.ensure((size_t)batch * dm * 4));
-    WV_TRY(m->x_lo.ensure((size_t)batch * dm * 4));
+    WV_TRY(m->x_hi.ensure((size_t)rows * dm * 4));
+    WV_TRY(m->x_lo.ensure((size_t)rows * dm * 4));
     WV_CUDA(split_tf32(static_cast<const float*>(xd), m->x_hi.as<float>(), m->x_lo.as<float>(),
-                       (int64_t)batch * dm, s), "split x");
+                       (int64_t)rows * dm, s), "split x");
     count_launch();
     q.a = m->x_hi.p;
     q.a_lo = m->x_lo.p;
   } else {
     q.a = xd;
   }
-  q.kv_k = kv->k_pool.p;
-  q.kv_v = kv->v_pool.p;
+  q.kv_k = kv->e4m3 ? nullptr : kv->k_pool.p;
+  q.kv_v = kv->e4m3 ? nullptr : kv->v_pool.p;
   q.kv_slot = m->slots.as<int>();
   q.kv_col0 = m->qd_l;
   q.kv_dim = m->kd_l;
@@ -1212,7 +1329,11 @@ Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* pos
   prof_begin(kProfGemmQkvDecode, s);
   WV_TRY(run_proj(m, q, s, &kv_done));
   prof_end(kProfGemmQkvDecode, s);
-  if (!kv_done) {
+  if (kv->e4m3) {
+    const char* base = static_cast<const char*>(m->qkv.p);
+    WV_TRY(kv8_append_rows(kv, batch, seq, base + (size_t)m->qd_l * es, base + (size_t)(m->qd_l + m->kd_l) * es,
+                           m->nqkv, s));
+  } else if (!kv_done) {
     const char* base = static_cast<const char*>(m->qkv.p);
     WV_CUDA(kv_append(base + (size_t)m->qd_l * es, base + (size_t)(m->qd_l + m->kd_l) * es, m->nqkv, batch,
                       m->kd_l, c.hd, f32 ? 0 : 1, m->slots.as<int>(), kv->k_pool.p, kv->v_pool.p, s),
@@ -1222,42 +1343,62 @@ Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* pos
 
   void* attn = pre;
   if (!attn || !on_device) {
-    WV_TRY(m->attn.ensure((size_t)batch * m->qd_l * es));
+    WV_TRY(m->attn.ensure((size_t)rows * m->qd_l * es));
     attn = m->attn.p;
   }
-  DecodeArgs d;
-  d.q = m->qkv.p;
-  d.ldq = m->nqkv;
-  d.k_pool = kv->k_pool.p;
-  d.v_pool = kv->v_pool.p;
-  d.block_table = kv->block_table.as<int>();
-  d.max_pages = kv->pages_per_seq;
-  d.ctx_len = kv->ctx_len.as<int>();
-  d.out = attn;
-  d.ldo = m->qd_l;
-  d.is_bf16 = f32 ? 0 : 1;
-  d.batch = batch;
-  d.num_heads = m->hc;
-  d.num_kv_heads = m->khc;
-  d.head_dim = c.hd;
-  d.alibi = c.alibi;
-  d.sigmoid = c.c.softmax == 1;
-  d.head_base = m->h0;
-  d.total_heads = c.c.num_heads;
-  d.scale = c.scale;
-  d.max_ctx = max_ctx + 1;
-  d.pool_rows = (int64_t)kv->max_batch * kv->pages_per_seq * m->khc * kPageTokens;
-  d.err = m->dev->err;
-  d.sm_count = m->dev->sm_count;
-  WV_TRY(kv->scratch.ensure(decode_scratch_floats(d) * 4));
-  d.partial = kv->scratch.as<float>();
-  prof_begin(kProfAttnDecode, s);
-  WV_CUDA(attn_decode(d, s), "attn_decode");
-  prof_end(kProfAttnDecode, s);
-  count_launch(2);
+  if (kv->e4m3) {
+    Kv8AttnArgs a;
+    a.c = kv8_args(kv);
+    a.batch = batch;
+    a.seq = seq;
+    a.heads = m->hc;
+    a.max_ctx = max_ctx + seq;
+    a.q = m->qkv.p;
+    a.ldq = m->nqkv;
+    a.out = attn;
+    a.ldo = m->qd_l;
+    kv8_mask(c, &a);
+    a.err = m->dev->err;
+    a.sm_count = m->dev->sm_count;
+    prof_begin(kProfAttnDecode, s);
+    WV_CUDA(kv8_attention(a, s), "kv8 attention");
+    prof_end(kProfAttnDecode, s);
+    count_launch();
+  } else {
+    DecodeArgs d;
+    d.q = m->qkv.p;
+    d.ldq = m->nqkv;
+    d.k_pool = kv->k_pool.p;
+    d.v_pool = kv->v_pool.p;
+    d.block_table = kv->block_table.as<int>();
+    d.max_pages = kv->pages_per_seq;
+    d.ctx_len = kv->ctx_len.as<int>();
+    d.out = attn;
+    d.ldo = m->qd_l;
+    d.is_bf16 = f32 ? 0 : 1;
+    d.batch = batch;
+    d.num_heads = m->hc;
+    d.num_kv_heads = m->khc;
+    d.head_dim = c.hd;
+    d.alibi = c.alibi;
+    d.sigmoid = c.c.softmax == 1;
+    d.head_base = m->h0;
+    d.total_heads = c.c.num_heads;
+    d.scale = c.scale;
+    d.max_ctx = max_ctx + 1;
+    d.pool_rows = (int64_t)kv->max_batch * kv->pages_per_seq * m->khc * kPageTokens;
+    d.err = m->dev->err;
+    d.sm_count = m->dev->sm_count;
+    WV_TRY(kv->scratch.ensure(decode_scratch_floats(d) * 4));
+    d.partial = kv->scratch.as<float>();
+    prof_begin(kProfAttnDecode, s);
+    WV_CUDA(attn_decode(d, s), "attn_decode");
+    prof_end(kProfAttnDecode, s);
+    count_launch(2);
+  }
 
   Proj o;
-  o.M = batch;
+  o.M = rows;
   o.K = m->qd_l;
   o.lda = m->qd_l;
   o.N = dm;
@@ -1268,10 +1409,10 @@ Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* pos
   o.w_scale = m->wo_scale.as<float>();
   o.splitk = true;
   if (f32) {
-    WV_TRY(m->attn_hi.ensure((size_t)batch * m->qd_l * 4));
-    WV_TRY(m->attn_lo.ensure((size_t)batch * m->qd_l * 4));
+    WV_TRY(m->attn_hi.ensure((size_t)rows * m->qd_l * 4));
+    WV_TRY(m->attn_lo.ensure((size_t)rows * m->qd_l * 4));
     WV_CUDA(split_tf32(static_cast<const float*>(attn), m->attn_hi.as<float>(), m->attn_lo.as<float>(),
-                       (int64_t)batch * m->qd_l, s), "split attn");
+                       (int64_t)rows * m->qd_l, s), "split attn");
     count_launch();
     o.a = m->attn_hi.p;
     o.a_lo = m->attn_lo.p;
@@ -1282,22 +1423,22 @@ Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* pos
   WV_TRY(run_proj(m, o, s));
   prof_end(kProfGemmODecode, s);
   if (m->comm) {
-    // The decode output (batch x d_model) is small: one peer-memory kernel over
+    // The decode output (rows x d_model) is small: one peer-memory kernel over
     // NVLink instead of NCCL when the layer can take it.
-    const size_t count = (size_t)batch * dm;
+    const size_t count = (size_t)rows * dm;
     prof_begin(kProfAllReduce, s);
     if (comm_peer_ok(m, count * es)) WV_TRY(comm_peer_allreduce(m, postd, count, !f32, s));
     else WV_TRY(comm_allreduce(m, postd, count, !f32, s));
     prof_end(kProfAllReduce, s);
   }
-  for (int b = 0; b < batch; ++b) kv->ctx_host[b] += 1;
+  for (int b = 0; b < batch; ++b) kv->ctx_host[b] += seq;
   if (!on_device) {
     // pageable outputs with a communicator: copy only after the bounded wait (see
     // mha_forward)
     const bool defer_d2h = m->comm && m->nranks > 1 && (!host_pinned(post) || !host_pinned(pre));
     if (defer_d2h) WV_TRY(comm_wait(m, s, "decode"));
-    WV_CUDA(cudaMemcpyAsync(post, postd, (size_t)batch * dm * es, cudaMemcpyDeviceToHost, s), "D2H post");
-    if (pre) WV_CUDA(cudaMemcpyAsync(pre, attn, (size_t)batch * m->qd_l * es, cudaMemcpyDeviceToHost, s), "D2H pre");
+    WV_CUDA(cudaMemcpyAsync(post, postd, (size_t)rows * dm * es, cudaMemcpyDeviceToHost, s), "D2H post");
+    if (pre) WV_CUDA(cudaMemcpyAsync(pre, attn, (size_t)rows * m->qd_l * es, cudaMemcpyDeviceToHost, s), "D2H pre");
     WV_TRY(comm_wait(m, s, "decode"));
     WV_TRY(check_device_error(m->dev));
   }

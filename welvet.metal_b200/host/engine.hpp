@@ -163,6 +163,11 @@ struct Mha {
   DevBuf splitk_ws;  // split-K partial sums of the decode projections
   DevBuf qkv_hi, qkv_lo;  // FP32 path: TF32 split of q/k/v for the 3xTF32 attention
   DevBuf attn_ctr;        // tile counter of the persistent prefill attention (one int)
+  // RMS norm of every query and key head before the position encoding
+  // (welvet_b200_mha_set_qk_norm): gammas [queries, keys][head_dim]
+  bool qk_norm = false;
+  float qk_eps = 1e-6f;
+  DevBuf qk_gamma;
   // communicator (head-sharded tensor parallelism); the all-reduce of a forward
   // chunk runs on comm_stream while the next chunk computes on the caller's stream
   void* comm = nullptr;
@@ -230,16 +235,23 @@ Status mha_forward(Mha* m, int batch, int seq, const void* x, void* pre, void* p
 // (ranks in order); the input rows are all-gathered and the output rows
 // reduce-scattered over NVLink, so each GPU copies 1/N of them over PCIe.
 
+Status mha_set_qk_norm(Mha* m, double eps, const float* q_gamma, const float* k_gamma, bool on_device);
+
 struct Kv {
   Mha* layer = nullptr;
   int max_batch = 0, max_ctx = 0, pages_per_seq = 0;
+  // E4M3 codes in pages of kKv8Page tokens, a scale per block of kKv8Block; otherwise the
+  // layer's precision in pages of kPageTokens
+  bool e4m3 = false;
+  DevBuf k_scale, v_scale;
   DevBuf k_pool, v_pool, block_table, ctx_len, scratch;
   std::vector<int> ctx_host;
 };
-Status kv_create(Mha* m, int max_batch, int max_ctx, Kv** out);
+Status kv_create(Mha* m, int max_batch, int max_ctx, bool e4m3, Kv** out);
 Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on_device,
                cudaStream_t s);
-Status mha_decode(Mha* m, Kv* kv, int batch, const void* x, void* pre, void* post,
+// One step of seq new tokens per sequence (seq > 1: E4M3 caches only).
+Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, void* post,
                   bool on_device, cudaStream_t s);
 
 // Attention over an E4M3 cache (kv8.cpp): whether the configuration is built (code 2
@@ -300,6 +312,8 @@ void comm_release(Mha* m);
 cudaError_t make_prefill_slots(int* slots, int batch, int seq, int pages_per_seq, cudaStream_t s);
 cudaError_t make_decode_rows(int* ctx, int* positions, int* slots, int batch, int pages_per_seq,
                              cudaStream_t s);
+// positions[b * seq + t] = ctx[b] + t; ctx[b] += seq
+cudaError_t make_extend_rows(int* ctx, int* positions, int batch, int seq, cudaStream_t s);
 cudaError_t set_ctx(int* ctx, int batch, int value, cudaStream_t s);
 cudaError_t make_block_table(int* bt, int batch, int pages_per_seq, cudaStream_t s);
 

@@ -24,6 +24,13 @@ __global__ void decode_rows_kernel(int* ctx, int* positions, int* slots, int bat
   ctx[b] = L + 1;
 }
 
+__global__ void extend_rows_kernel(int* ctx, int* positions, int seq) {
+  const int b = blockIdx.x, L = ctx[b];
+  for (int t = threadIdx.x; t < seq; t += blockDim.x) positions[(int64_t)b * seq + t] = L + t;
+  __syncthreads();  // every thread has read the old length
+  if (threadIdx.x == 0) ctx[b] = L + seq;
+}
+
 __global__ void set_ctx_kernel(int* ctx, int batch, int value) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b < batch) ctx[b] = value;
@@ -45,6 +52,10 @@ cudaError_t make_prefill_slots(int* slots, int batch, int seq, int pps, cudaStre
 }
 cudaError_t make_decode_rows(int* ctx, int* positions, int* slots, int batch, int pps, cudaStream_t s) {
   decode_rows_kernel<<<(batch + 127) / 128, 128, 0, s>>>(ctx, positions, slots, batch, pps);
+  return cudaGetLastError();
+}
+cudaError_t make_extend_rows(int* ctx, int* positions, int batch, int seq, cudaStream_t s) {
+  extend_rows_kernel<<<batch, 128, 0, s>>>(ctx, positions, seq);
   return cudaGetLastError();
 }
 cudaError_t set_ctx(int* ctx, int batch, int value, cudaStream_t s) {

@@ -46,7 +46,8 @@ EXT_SYMBOLS = ("welvet_b200_mha_config_default", "welvet_b200_mha_mount", "welve
                "welvet_b200_embedding_forward", "welvet_b200_wait_probe", "welvet_b200_mha_set_output_mode",
                "welvet_b200_attention_tf32", "welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward",
                "welvet_b200_qk_norm_rope_workspace", "welvet_b200_qk_norm_rope_backward", "welvet_b200_kv8_append",
-               "welvet_b200_kv8_attention")
+               "welvet_b200_kv8_attention", "welvet_b200_kv_create_e4m3", "welvet_b200_mha_extend",
+               "welvet_b200_mha_set_qk_norm")
 PROFILE_SLOTS = ("gemm_qkv", "attn_prefill", "gemm_o", "attn_decode", "gemm_qkv_decode", "gemm_o_decode",
                  "allreduce", "other", "gemm_gate_up", "gemm_down", "norm", "embedding", "attn_bwd", "gemm_grad")
 
@@ -183,7 +184,11 @@ def lib():
     L.welvet_b200_qk_norm_rope_backward.argtypes = norm + [_vp, C.c_int64] * 2 + [_vp] * 3 + [C.c_int32, _vp]
     L.welvet_b200_kv8_append.argtypes = [kv8p, C.c_int32, _vp, _vp, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, _vp]
     L.welvet_b200_kv8_attention.argtypes = [cfgp, kv8p, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, _vp]
-    for name in ("welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward", "welvet_b200_qk_norm_rope_backward",
+    L.welvet_b200_kv_create_e4m3.argtypes = [_vp, C.c_int32, C.c_int32, C.POINTER(_vp)]
+    L.welvet_b200_mha_extend.argtypes = [_vp, _vp, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int32, _vp]
+    L.welvet_b200_mha_set_qk_norm.argtypes = [_vp, C.c_double, _vp, _vp, C.c_int32]
+    for name in ("welvet_b200_kv_create_e4m3", "welvet_b200_mha_extend", "welvet_b200_mha_set_qk_norm",
+                 "welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward", "welvet_b200_qk_norm_rope_backward",
                  "welvet_b200_kv8_append", "welvet_b200_kv8_attention",
                  "welvet_b200_wait_probe", "welvet_b200_mha_set_output_mode", "welvet_b200_attention_tf32",
 "welvet_b200_mha_mount", "welvet_b200_mha_forward", "welvet_b200_mha_forward_rows",
@@ -468,6 +473,22 @@ class MhaLayer:
         check(lib().welvet_b200_mha_decode(self._h, kv.handle, batch, _ptr(x), _ptr(pre), _ptr(post),
                                            _on_device(x, pre, post), _stream(stream)))
 
+    def extend(self, kv: "KvCache", batch, seq, x, pre, post, stream=None):
+        """seq new tokens per sequence over an E4M3 cache (welvet_b200_mha_extend)."""
+        check(lib().welvet_b200_mha_extend(self._h, kv.handle, batch, seq, _ptr(x), _ptr(pre), _ptr(post),
+                                           _on_device(x, pre, post), _stream(stream)))
+
+    def set_qk_norm(self, q_gamma, k_gamma, eps=1e-6):
+        """RMS norm of every query and key head before the position encoding, gammas
+        [head_dim]; None, None: no norm (welvet_b200_mha_set_qk_norm)."""
+        on_dev = _on_device(q_gamma, k_gamma)
+        if q_gamma is not None and not on_dev:
+            q_gamma, k_gamma = (np.ascontiguousarray(a, dtype=np.float32) for a in (q_gamma, k_gamma))
+        for g in (q_gamma, k_gamma):
+            if g is not None and (g.shape != (self.head_dim,) or "float32" not in str(g.dtype)):
+                raise ValueError(f"gammas of {self.head_dim} FP32 values expected")
+        check(lib().welvet_b200_mha_set_qk_norm(self._h, eps, _ptr(q_gamma), _ptr(k_gamma), on_dev))
+
     def set_output_mode(self, mode: int):
         """0: all-reduce output (default); 1: reduce-scatter, rank r keeps the r-th
         row slice of each chunk summed; 2: the same rows through an exchange of the
@@ -480,10 +501,14 @@ class MhaLayer:
 
 
 class KvCache:
-    def __init__(self, layer: MhaLayer, max_batch: int, max_ctx: int):
+    """Paged KV cache of a layer; e4m3: 8-bit codes with a scale per 16 tokens and head
+    (welvet_b200_kv_create_e4m3)."""
+
+    def __init__(self, layer: MhaLayer, max_batch: int, max_ctx: int, e4m3: bool = False):
         self._h = _vp()
         self.layer = layer
-        check(lib().welvet_b200_kv_create(layer.handle, max_batch, max_ctx, C.byref(self._h)))
+        create = lib().welvet_b200_kv_create_e4m3 if e4m3 else lib().welvet_b200_kv_create
+        check(create(layer.handle, max_batch, max_ctx, C.byref(self._h)))
 
     @property
     def handle(self):
