@@ -532,12 +532,19 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     uint64_t l2[CPW / 2];  // sums of the columns, in pairs
 #pragma unroll
     for (int c = 0; c < CPW / 2; ++c) l2[c] = 0ull;
+    int slot = tg;  // of the scales' ring, and its pass
+    uint32_t pass = 0;
     for (int i = tg; i < tiles; i += NTG) {
       const int base = base0 + i * kKeys, kpos = base + key;
       // After a wait that gave up, the tiles are still walked (the waits return at once):
       // the warpgroup's barriers need every thread.
-      ok = mbar_wait(&sc_full[i % T::SCALES], (i / T::SCALES) & 1, abort_flag, a.err, kErrWaitFull) && ok;
-      const uint32_t sc = sm + T::OFF_SC + (i % T::SCALES) * 64 + (key >> 4) * 4;
+      ok = mbar_wait(&sc_full[slot], pass, abort_flag, a.err, kErrWaitFull) && ok;
+      const uint32_t sc = sm + T::OFF_SC + slot * 64 + (key >> 4) * 4;
+      slot += NTG;
+      if (slot >= T::SCALES) {
+        slot -= T::SCALES;
+        pass ^= 1;
+      }
       const bool on = kpos < k1;
       const float ks = lds(sc), vs = lds(sc + 32);
       float ev;
@@ -587,8 +594,8 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
       float top = fmaxf(y[0], y[1]);
 #pragma unroll
       for (int c = 2; c < CPW; c += 2) top = fmax3(top, y[c], y[c + 1]);
-      // P is free (and, with two tile groups, this group's O holds all its tiles)
-      if (i >= 2) ok = mbar_wait(&pv_done[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+      // S_i was committed behind PV_{i-2}, so P's buffer is free (and, with two tile groups,
+      // this group's O holds all its tiles).
       if (wg_any<NCG * NTG>(wg, !known || top > kBias + kSlack)) {
         // new references: the maximum of every column over the tile's keys
 #pragma unroll
