@@ -332,7 +332,8 @@ WELVET_API welvet_status welvet_b200_qk_norm_rope_backward(
  * tokens of a KV head: value = code * scale. All pointers are device memory of the
  * caller (codes 16-byte aligned for the tensor-core kernel).
  *   k, v            codes [pages][kv_heads][64][head_dim]
- *   k_scale, v_scale  [pages][kv_heads][4], positive; append writes powers of two
+ *   k_scale, v_scale  [pages][kv_heads][4], positive (NaN: the block reads as NaN);
+ *                   append writes powers of two from 2^-64 to 2^120
  *   block_table     [batch][max_pages] page ids; entry j holds tokens [64j, 64j+64)
  *   ctx_len         [batch] tokens of each sequence INCLUDING the new ones of the call
  * head_dim even, at most 256. */
@@ -366,8 +367,9 @@ WELVET_API welvet_status welvet_b200_kv8_append(const welvet_b200_kv8_cache* cac
  * cfg: num_heads, num_kv_heads, head_dim, scale_override, mask, window, ALiBi (pos 2 or
  * 3), head shard, precision 1; q and out are BF16 rows, ldq / ldo apart. Rows that see
  * nothing (t >= n_b, an empty sequence) are zero. max_ctx bounds ctx_len (it sizes the
- * split of long contexts, not the result's meaning). Code 2 for sigmoid scores, other
- * masks and FP32 layers. */
+ * split of long contexts, not the result's meaning). Probabilities are rounded to a
+ * relative 2^-9, and below 2^-19 of the row's largest to 2^-28 of it. Code 2 for sigmoid
+ * scores, other masks and FP32 layers. */
 WELVET_API welvet_status welvet_b200_kv8_attention(const welvet_b200_mha_config* cfg,
                                                    const welvet_b200_kv8_cache* cache, int32_t seq,
                                                    const int32_t* seq_lens, int32_t max_ctx, const void* q,

@@ -291,6 +291,42 @@ def test_attention(torch_cuda, batch, seq, ctx, heads, kv, hd, kind):
     assert _close(out, *_reference(torch, cache, cfg, seq, q))
 
 
+@pytest.mark.parametrize("hd,kv,seq", [(64, 8, 1), (64, 8, 5), (64, 4, 16), (128, 8, 1), (128, 8, 3), (128, 4, 12)])
+def test_attention_full_gpu(torch_cuda, hd, kv, seq):
+    """More sequences than fit the GPU at once, lengths that end anywhere in a tile, NaN
+    codes behind their ends, five times over. Keys of zeros make every probability the
+    same power of two and small integers make every sum exact, so a row is the mean of
+    its values up to the quotient's and the output's rounding."""
+    torch = torch_cuda
+    batch, heads, most = 96, 4 * kv, 3700
+    ctx = [most - (b * 389) % 700 for b in range(batch)]
+    cache = _cache(torch, batch, ctx, kv, hd, seed=1)
+    keys, values, ks, vs, table, lens = cache.tensors
+    table, lens = table.long(), lens.long()
+    for x in (ks, vs):
+        x.fill_(1.0)
+    at = torch.arange(table.shape[1] * PAGE, device="cuda")
+    val = 1 + (at[:, None] // 48 + torch.arange(hd, device="cuda")) % 7      # [token][hd]
+    code = val.float().to(torch.float8_e4m3fn).view(torch.uint8)
+    for b in range(batch):
+        past = (at >= ctx[b])[:, None]
+        for c, x in ((keys, torch.zeros_like(code)), (values, code)):
+            x = torch.where(past, 0x7f, x).view(-1, 1, PAGE, hd)
+            used = (ctx[b] + PAGE - 1) // PAGE
+            c[table[b, :used]] = x[:used].expand(-1, kv, -1, -1)
+    pos = lens[:, None] - seq + torch.arange(seq, device="cuda")              # [batch][seq]
+    sums = torch.cumsum(val.double(), 0)
+    o = (sums[pos] / (pos + 1)[..., None]).view(batch * seq, 1, hd)
+    q = torch.randn(batch * seq, heads * hd, device="cuda").bfloat16()
+    out = torch.empty_like(q)
+    for _ in range(5):
+        out.fill_(7)
+        W.kv8_attention(_config(heads, kv, hd), cache, seq, q, out, most)
+        W.device_check()
+        d = (out.double().view(batch * seq, heads, hd) - o).abs()
+        assert bool((d <= (2.0 ** -8 + 2.0 ** -20) * o).all())
+
+
 @pytest.mark.parametrize("hd", [64, 128, 48])
 @pytest.mark.parametrize("seq", [1, 4, 70])
 def test_attention_unequal_lengths_and_empty_rows(torch_cuda, hd, seq):

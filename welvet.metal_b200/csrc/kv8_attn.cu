@@ -22,7 +22,8 @@
 // Scores and sums are FP32 (TMEM accumulators, registers).
 //
 // Softmax in the log2 domain with the value scale folded in: z = s kscale qscale
-// scale log2e + log2(vscale), p = 2^(z - ref), O += p * code, l += p / vscale. ref is a
+// scale log2e + log2(vscale), p = 2^(z - ref), O += p * code, l += p / vscale (FP32: the
+// scales of a row's blocks may lie 2^100 apart). ref is a
 // column's running maximum of z, raised only when some p would exceed 2^10 (E5M2 has the
 // room), so that after the first tile one vote and no maximum is the rule; when it
 // moves, O and l are rescaled.
@@ -455,11 +456,11 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
           pv_mma(i, kk);
           if (both && kk < kS) s_mma(j, kk);
         }
+        umma_commit(&pv_done[i & 1]);
         if (both) {
           umma_commit(&s_full[j & 1]);
           umma_commit(&k_empty[j % KST]);
         }
-        umma_commit(&pv_done[i & 1]);
         umma_commit(&v_empty[i % VST]);
       }
       __syncwarp();
@@ -550,13 +551,16 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
       float ev;
       asm("lg2.approx.f32 %0, %1;" : "=f"(ev) : "f"(vs));
       const float inv = on && vs == vs ? __fdividef(1.f, vs) : 0.f;
-      if (!on && c0 == 0) {  // rows past the context may hold NaN codes: 0 * NaN
+      ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
+      // Rows past the context may hold NaN codes, and 0 * NaN is NaN: cleared, now that
+      // S_i has come and PV_{i-2}, the last reader of an earlier tile in this slot, is done.
+      if (!on && c0 == 0) {
         ok = mbar_wait(&v_full[i % VST], (i / VST) & 1, abort_flag, a.err, kErrWaitFull) && ok;
         const uint32_t row = sm + T::OFF_V + (i % VST) * T::TILE + key * HD;
 #pragma unroll 1
         for (int x = 0; x < HD; x += 16) sts4(row + x, 0u, 0u, 0u, 0u);
       }
-      ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
+      __syncwarp();  // lanes leave a wait one by one; the TMEM loads need them together
       tc_fence_after();
       // y of this key for the group's columns: z + bias - ref (ref = bias before the first)
       float y[CPW];
@@ -613,6 +617,7 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
         }
         if (NTG == 1 && i > 0)
           ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+        __syncwarp();
         tc_fence_after();
         wg_sync<NCG * NTG>(wg);
         if (key < CPW) {
@@ -836,7 +841,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8AttnAr
   // 8 pairs of 32768 keys (head_dim 128) take 179 us unsplit, 28 in clusters of 8, 19 in
   // clusters of 16; 128 pairs of 4096 keys (head_dim 64) 28, and 17 in clusters of 4;
   // 512 pairs of them 48, and 52 in clusters of 2, which no longer fit at once.
-  const int keys = a.window > 0 ? std::min(a.max_ctx, a.window + a.seq + kKv8Page) : a.max_ctx;
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + a.seq + kKv8Page) : a.max_ctx;
   const int64_t slots = (int64_t)a.sm_count * T::PER_SM;
   int k = 0;
   while (k < kMaxLog && pairs << (k + 1) <= slots * kResident[T::PER_SM > 1][k + 1] / 1000 && (kKeys << (k + 1)) <= keys) ++k;
