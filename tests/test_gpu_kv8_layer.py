@@ -185,6 +185,19 @@ def test_norm_in_the_forward_of_fp32_layers(torch_cuda, hd, rope):
     assert torch.equal(plain, again) and not torch.equal(plain, post)
 
 
+def test_lengths_without_rows_read_zeros(torch_cuda):
+    torch = torch_cuda
+    cfg = W.MhaConfig.make(128, 4, 2, head_dim=64, precision=1, max_seq_len=256)
+    layer = W.MhaLayer(cfg, *W.xavier_weights(128, 256, 128, 0))
+    cache = W.KvCache(layer, 2, 200, e4m3=True)
+    cache.fill(2, 150)
+    x = torch.randn(2, 128, device="cuda").bfloat16()
+    pre, post = torch.empty(2, 256, device="cuda", dtype=torch.bfloat16), torch.empty_like(x)
+    layer.decode(cache, 2, x, pre, post)
+    layer.check_device()
+    assert bool(torch.isfinite(pre.float()).all()) and float(pre.abs().max()) < 1.0  # one row in 151 is not zero
+
+
 def test_refusals(torch_cuda):
     torch = torch_cuda
     d, heads, kv, hd = 128, 4, 2, 32

@@ -1198,11 +1198,20 @@ Status kv_create(Mha* m, int max_batch, int max_ctx, bool e4m3, Kv** out) {
   const size_t pool = (size_t)max_batch * kv->pages_per_seq * page * m->kd_l * es;
   if (e4m3) {
     const size_t scales = (size_t)max_batch * kv->pages_per_seq * m->khc * kKv8Subs * 4;
+    if (scales / 4 > INT32_MAX) return Status::err(1, "kv: max_batch or max_ctx too large");
     WV_TRY(kv->k_scale.ensure(scales));
     WV_TRY(kv->v_scale.ensure(scales));
   }
   WV_TRY(kv->k_pool.ensure(pool));
   WV_TRY(kv->v_pool.ensure(pool));
+  if (e4m3) {  // tokens whose length is set but which nobody wrote read as zeros: code 0, scale 1
+    const int n = (int)(kv->k_scale.bytes / 4);
+    WV_CUDA(cudaMemsetAsync(kv->k_pool.p, 0, pool, 0), "kv pool");
+    WV_CUDA(cudaMemsetAsync(kv->v_pool.p, 0, pool, 0), "kv pool");
+    WV_CUDA(set_ctx(kv->k_scale.as<int>(), n, 0x3f800000, 0), "kv scales");
+    WV_CUDA(set_ctx(kv->v_scale.as<int>(), n, 0x3f800000, 0), "kv scales");
+    count_launch(2);
+  }
   WV_TRY(kv->block_table.ensure((size_t)max_batch * kv->pages_per_seq * 4));
   WV_TRY(kv->ctx_len.ensure((size_t)max_batch * 4));
   WV_CUDA(make_block_table(kv->block_table.as<int>(), max_batch, kv->pages_per_seq, 0), "block table");
