@@ -92,49 +92,96 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const Kv8AppendArgs a) 
   if (threadIdx.x == 0) *scale = s;
 }
 
+// The largest magnitude of three values, NaN if one is NaN.
+WV_DEV float abs_max(float x, float y, float z) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+// e4m3x2(lo f, hi f), both products in one instruction.
+WV_DEV uint32_t e4m3x2_scaled(float lo, float hi, float f) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(lo), "+f"(hi) : "f"(f));
+  return e4m3x2(lo, hi);
+}
+
 // head_dim 64 and 128, 16-byte aligned rows, codes and table: one warp per (block, KV
 // head, K or V) holds the block's 16 rows in registers, 8 pairs of a row per lane (16
 // bytes of each half, the partners of the rotation together), so the rows are read
 // once and the maximum needs five shuffles. Bound by HBM for prompts (4 bytes read, 2
 // written a value pair of K and V), by latency for single tokens.
-constexpr int kAppendWarps = 4;  // a CTA's warps: 117 us with 8 for 4 x 4096 tokens x 32 heads of 128, 94 with 4
+// CTAs of 4 heads, 24 warps to an SM: 4 x 4096 tokens x 32 KV heads of 128 take 73 us
+// (5.4 TB/s of 403 MB); 8 heads 80 us, 2 heads 107 us, 20 warps without the bound on
+// registers 87 us; values without a rotation 64 us.
+constexpr int kAppendWarps = 4;
 template <int HD>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_vec_kernel(const Kv8AppendArgs a, int blocks) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 6) kv8_append_vec_kernel(const Kv8AppendArgs a, int blocks) {
   constexpr int LPR = HD / 16, RPW = 32 / LPR, IT = kKv8Block / RPW;
+  constexpr int F4 = HD / 4;  // 16-byte pieces of a row of the table, two pairs each
+  __shared__ float4 tab[kKv8Block * F4];
   pdl_wait();
   pdl_trigger();
   const int lane = (int)lane_id(), sub = lane / LPR, at = (lane % LPR) * 8;
-  int64_t unit = (int64_t)blockIdx.x * kAppendWarps + warp_id();
-  const int kh = (int)(unit % a.c.kv_heads);  // neighbouring warps read neighbouring heads of the same rows
-  unit /= a.c.kv_heads;
+  const int groups = (a.c.kv_heads + (int)(blockDim.x >> 5) - 1) / (int)(blockDim.x >> 5);
+  int unit = (int)blockIdx.x / groups;
+  const int kh = ((int)blockIdx.x % groups) * (int)(blockDim.x >> 5) + (int)warp_id();
   const bool is_v = (unit & 1) != 0;
   unit >>= 1;
-  const int b = (int)(unit / blocks);
-  if (b >= a.batch) return;
+  const int b = unit / blocks;
   const int n = kv8_new(a.seq_lens, b, a.seq), ctx = a.c.ctx_len[b], start = ctx - n;
-  const int first = max(start, 0), blk = first / kKv8Block + (int)(unit % blocks);
+  const int first = max(start, 0), blk = first / kKv8Block + unit % blocks;
   const int p0 = blk * kKv8Block, lo = max(first, p0), hi = min(ctx, p0 + kKv8Block);
   if (lo >= hi) return;
-  const int page = kv8_page(a.c, b, blk / kKv8Subs, a.err);
-  if (page < 0) return;
-  const size_t ph = (size_t)page * a.c.kv_heads + kh;
-  uint8_t* codes = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + (ph * kKv8Page + p0 % kKv8Page) * HD + at;
-  float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + ph * kKv8Subs + blk % kKv8Subs;
   const int ld = is_v ? a.ldv : a.ldk;
   const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(is_v ? a.v : a.k) + (size_t)kh * HD + at;
-  const float s_old = lo > p0 ? *scale : 0.f;
-
   uint4 raw[IT][2];
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int p = p0 + it * RPW + sub;
     raw[it][0] = raw[it][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (p < lo || p >= hi) continue;
+    if (p < lo || p >= hi || kh >= a.c.kv_heads) continue;
     const __nv_bfloat16* x = src + ((size_t)b * a.seq + (p - start)) * ld;
     raw[it][0] = *reinterpret_cast<const uint4*>(x);
     raw[it][1] = *reinterpret_cast<const uint4*>(x + HD / 2);
   }
-  float x[IT][2][8], amax = 0.f;
+  // A lane's eight pairs are four pieces of the table, 64 bytes apart between lanes: read
+  // from global memory that is four times the wavefronts. The CTA's heads share the
+  // block's rows of it in shared memory, pieces swapped so that no bank meets another.
+  const bool rotate = !is_v && a.rope;
+  if (rotate) {
+    const float4* src4 = reinterpret_cast<const float4*>(a.rope);
+    for (int i = (lo - p0) * F4 + (int)threadIdx.x; i < (hi - p0) * F4; i += (int)blockDim.x) {
+      const int p = p0 + i / F4;
+      if (p < a.max_pos)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&tab[i ^ ((i >> 3) & 3)])),
+                     "l"(src4 + (size_t)p * F4 + i % F4)
+                     : "memory");
+      else if (a.err)
+        atomicCAS(a.err, 0u, kErrRopePos);
+    }
+  }
+  const int page = kv8_page(a.c, b, blk / kKv8Subs, a.err);
+  if (rotate) asm volatile("cp.async.wait_all;" ::: "memory");
+  if (page < 0) return;
+  __syncthreads();
+  if (kh >= a.c.kv_heads) return;
+  const size_t ph = (size_t)page * a.c.kv_heads + kh;
+  uint8_t* codes = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + (ph * kKv8Page + p0 % kKv8Page) * HD + at;
+  float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + ph * kKv8Subs + blk % kKv8Subs;
+  const float s_old = lo > p0 ? *scale : 0.f;
+
+  float x[IT][2][8], amax = 0.f;  // the largest magnitude; NaN if one is
+  if (!rotate) {                  // BF16 magnitudes order as integers, NaN above all
+    uint32_t top = 0u;
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        top = __vmaxu2(__vmaxu2(__vmaxu2(top, raw[it][hf].x & 0x7fff7fffu), raw[it][hf].y & 0x7fff7fffu),
+                       __vmaxu2(raw[it][hf].z & 0x7fff7fffu, raw[it][hf].w & 0x7fff7fffu));
+    amax = __uint_as_float(max(top & 0xffff0000u, top << 16));
+  }
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int p = p0 + it * RPW + sub;
@@ -147,12 +194,12 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_vec_kernel(const
         x[it][hf][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
     }
-    if (!is_v && a.rope && p >= lo && p < hi) {
-      if (p < a.max_pos) {
-        const float4* tab = reinterpret_cast<const float4*>(a.rope + (size_t)p * (HD / 2) + at);
+    if (rotate) {
+      if (p >= lo && p < hi && p < a.max_pos) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          const float4 c = tab[i / 2];
+          const int f = (it * RPW + sub) * F4 + at / 2 + i / 2;
+          const float4 c = tab[f ^ ((f >> 3) & 3)];
           const float cs[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -161,34 +208,29 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_vec_kernel(const
             x[it][1][i + e] = __fadd_rn(__fmul_rn(u, cs[2 * e + 1]), __fmul_rn(w, cs[2 * e]));
           }
         }
-      } else if (a.err) {
-        atomicCAS(a.err, 0u, kErrRopePos);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = abs_max(amax, x[it][0][i], x[it][1][i]);
     }
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float m = fabsf(x[it][hf][i]);
-        amax = fmaxf(amax, m < INFINITY ? m : INFINITY);  // NaN counts as infinite
-      }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const bool poison = amax == INFINITY || s_old != s_old;
+  for (int o = 16; o > 0; o >>= 1) amax = abs_max(amax, __shfl_xor_sync(0xffffffffu, amax, o), 0.f);
+  const bool poison = !(amax < INFINITY) || s_old != s_old;
   const float s = poison ? __uint_as_float(0x7fc00000u) : fmaxf(kv8_scale(amax), s_old);
   // s is a power of two between 2^-64 and 2^120 (or the caller's own larger scale):
   // multiplying by 1/s is dividing by s.
-  const float inv = poison ? 0.f : 1.f / s;
+  const float inv = 1.f / s;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int r = it * RPW + sub, p = p0 + r;
     if (p < lo || p >= hi) continue;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      uint32_t c[4];
+      uint32_t c[4] = {};
+      if (!poison) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = poison ? 0u : e4m3x2(x[it][hf][2 * i] * inv, x[it][hf][2 * i + 1] * inv);
+        for (int i = 0; i < 4; ++i) c[i] = e4m3x2_scaled(x[it][hf][2 * i], x[it][hf][2 * i + 1], inv);
+      }
       *reinterpret_cast<uint2*>(codes + (size_t)r * HD + hf * (HD / 2)) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
     }
   }
@@ -309,11 +351,12 @@ cudaError_t kv8_append(const Kv8AppendArgs& a, cudaStream_t s) {
   // blocks that seq tokens can touch, wherever they begin
   const int blocks = (a.seq + kKv8Block - 2) / kKv8Block + 1;
   const auto low = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
-  const int64_t ctas = ((int64_t)blocks * 2 * a.c.kv_heads * a.batch + kAppendWarps - 1) / kAppendWarps;
+  const int warps = std::min(a.c.kv_heads, kAppendWarps);
+  const int64_t ctas = (int64_t)blocks * 2 * a.batch * ((a.c.kv_heads + warps - 1) / warps);
   if ((a.c.head_dim == 64 || a.c.head_dim == 128) && a.ldk % 8 == 0 && a.ldv % 8 == 0 && !low(a.k) && !low(a.v) &&
       !low(a.c.k) && !low(a.c.v) && !low(a.rope) && ctas < (1ll << 31))
     return launch_pdl(a.c.head_dim == 64 ? kv8_append_vec_kernel<64> : kv8_append_vec_kernel<128>, dim3((unsigned)ctas),
-                      dim3(kAppendWarps * 32), 0, s, a, blocks);
+                      dim3(warps * 32), 0, s, a, blocks);
   return launch_pdl(kv8_append_kernel, dim3(blocks, 2 * a.c.kv_heads, a.batch), dim3(128), 0, s, a);
 }
 
