@@ -68,9 +68,13 @@ template <int HD, int RT> struct KT {
   static constexpr int SOFT_WARPS = NCG * NTG * 4;
   static constexpr int THREADS = SOFT_WARPS * 32 + 64;
   static constexpr int TILE = kKeys * HD;           // bytes of a K or V tile
-  static constexpr int NS = 2 * RT;                 // columns of S: hi | lo
+  static constexpr int NS = 2 * RT;                 // query rows: hi | lo
+  // Columns of S: hi | lo, from one MMA, added in registers; with 64 columns hi + lo, from
+  // two MMAs into one accumulator (there the softmax bounds, not the MMAs).
+  static constexpr bool SUM = RT == 64;
+  static constexpr int SC = SUM ? RT : NS;
   static constexpr int NO = RT == 8 ? 32 : 3 * RT;  // columns of O and P: three terms
-  static constexpr int O_COL = 2 * NS;              // TMEM: S_0 | S_1 | O of the tile groups
+  static constexpr int O_COL = 2 * SC;              // TMEM: S_0 | S_1 | O of the tile groups
   static constexpr int COLS = O_COL + NTG * NO;
   static constexpr int TMEM = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   // tiles of the K and of the V ring
@@ -204,7 +208,9 @@ template <int N> WV_DEV void wg_sync(int w) {
   else if (w == 2) bar_sync<3>();
   else bar_sync<4>();
 }
-template <int WARPS> WV_DEV void soft_sync() { asm volatile("barrier.cta.sync 5, %0;" ::"n"(WARPS * 32) : "memory"); }
+// The softmax warps wait for the MMA warp's part of the columns' values.
+template <int WARPS> WV_DEV void cols_sync() { asm volatile("barrier.cta.sync 5, %0;" ::"n"(WARPS * 32) : "memory"); }
+template <int WARPS> WV_DEV void cols_arrive() { asm volatile("barrier.cta.arrive 5, %0;" ::"n"(WARPS * 32) : "memory"); }
 // Two FP16 pairs to four E5M2 codes (nearest), and the FP16 values of codes 0, 1 and 2,
 // 3 of a word: an E5M2 code is the upper byte of the FP16 pattern of its value.
 WV_DEV uint32_t e5m2x4(__half2 u, __half2 w) {
@@ -306,19 +312,35 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   const int kh = blockIdx.y, r0 = (int)(blockIdx.x / splits) * RT;
   const int G = a.heads / a.c.kv_heads;
   constexpr int NQ = (RT + kSoftWarps - 1) / kSoftWarps;  // columns of a softmax warp
-  __nv_bfloat16 xq[NQ][HD / 32];
-  int tq[NQ], hq[NQ];
+  constexpr int QV = HD / 32;  // consecutive dims of a lane
+  uint32_t xq[NQ][QV / 2];
+  int tq = 0;  // lane k: the token of the warp's column k
   if (warp < kSoftWarps) {
+    const bool wide = (reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.ldq * 2) % (2 * QV) == 0;
+    const int c = warp + lane % NQ * kSoftWarps;
+    tq = (r0 + c) / G;
+    const int64_t at = ((int64_t)b * a.seq + tq) * a.ldq + (int64_t)(kh * G + (r0 + c) - tq * G) * HD;
+    const bool there = c < RT && tq < a.seq;
 #pragma unroll
     for (int k = 0; k < NQ; ++k) {
-      const int c = warp + k * kSoftWarps;
-      tq[k] = (r0 + c) / G;
-      hq[k] = kh * G + (r0 + c) - tq[k] * G;
-      const __nv_bfloat16* q =
-          static_cast<const __nv_bfloat16*>(a.q) + ((size_t)b * a.seq + tq[k]) * a.ldq + (size_t)hq[k] * HD;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + __shfl_sync(0xffffffffu, at, k);
+      const uint16_t* x = reinterpret_cast<const uint16_t*>(q) + lane * QV;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i)
-        xq[k][i] = c < RT && tq[k] < a.seq ? q[lane + 32 * i] : __nv_bfloat16(0.f);
+      for (int i = 0; i < QV / 2; ++i) xq[k][i] = 0u;
+      if (__shfl_sync(0xffffffffu, there, k)) {
+        if (wide) {
+          if constexpr (QV == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(x);
+            xq[k][0] = v.x;
+            xq[k][1] = v.y;
+          } else {
+            xq[k][0] = *reinterpret_cast<const uint32_t*>(x);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < QV / 2; ++i) xq[k][i] = x[2 * i] | (uint32_t)x[2 * i + 1] << 16;
+        }
+      }
     }
   }
   const int n = kv8_new(a.seq_lens, b, a.seq);
@@ -409,8 +431,22 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     constexpr uint32_t HI_KV = desc_hi(8 * HD, kRow);       // 8 keys of HD bytes
     constexpr uint32_t HI_Q = desc_hi(128, 0);              // 8 rows of 16 bytes
     constexpr uint32_t HI_P = desc_hi(kKeys * 16, 0);       // 16 columns of every key
-    constexpr uint32_t IDESC_S = idesc_f8(0, 0, 128, T::NS, 0, 0);
+    constexpr uint32_t IDESC_S = idesc_f8(0, 0, 128, T::SC, 0, 0);
     constexpr uint32_t IDESC_PV = idesc_f8(0, 1, HD, T::NO, 1, 1);
+    for (int c = lane; c < RT; c += 32) {  // the columns' values, while it has nothing to issue
+      const int t = (r0 + c) / G, h = kh * G + (r0 + c) - t * G;
+      const bool live = t >= t0 && t <= t1;
+      for (int g = 0; g < NTG; ++g) {
+        refs[g * RT + c] = 0.f;
+        haves[g * RT + c] = 0.f;
+      }
+      // a column without a query sees whatever there is; its output is zero, or none
+      qhi[c] = live ? min(shift + t, k1 - 1) : k1 - 1;
+      outs[c] = t >= a.seq ? -1 : (((int64_t)b * a.seq + t) * a.ldo + (int64_t)h * HD) * 2 + (live ? 1 : 0);
+      if (ALIBI) slope[c] = exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * kLog2e;
+    }
+    __syncwarp();
+    cols_arrive<kSoftWarps + 1>();
     const uint32_t base = smem_u32(smem);
     const uint32_t q_lo = sdesc_lo(base + T::OFF_Q, T::NS * 16);
     const bool lead = elect_one();
@@ -420,8 +456,9 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     // S_j: HD / 32 MMAs; PV_i: kKeys / 32. An MMA waits for the one before it on the
     // same accumulator, so PV_i and S_{i+2} are issued in turn when both can run.
     const auto s_mma = [&](int j, int kk) {
-      umma_f8(tmem + (uint32_t)((j & 1) * T::NS), sdesc_lo(base + (j % KST) * T::TILE, 16) + kk * 2, HI_KV,
-              q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
+      const uint32_t s_col = tmem + (uint32_t)((j & 1) * T::SC), k_lo = sdesc_lo(base + (j % KST) * T::TILE, 16) + kk * 2;
+      umma_f8(s_col, k_lo, HI_KV, q_lo + kk * 2 * T::NS, HI_Q, IDESC_S, kk > 0);
+      if (T::SUM) umma_f8(s_col, k_lo, HI_KV, q_lo + kk * 2 * T::NS + RT, HI_Q, IDESC_S, 1);
     };
     const auto pv_mma = [&](int i, int kk) {
       umma_f8(tmem + T::O_COL + (i % NTG) * T::NO, sdesc_lo(base + T::OFF_V + (i % VST) * T::TILE, 16) + kk * (32 * HD / 16),
@@ -483,43 +520,42 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     for (int k = 0; k < NQ; ++k) {
       const int c = warp + k * kSoftWarps;
       if (c >= RT) break;
-      const int t = tq[k], h = hq[k];
+      const int t = __shfl_sync(0xffffffffu, tq, k);
       const bool live = t >= t0 && t <= t1;
-      float x[HD / 32], m = 0.f;
+      float x[QV], m = 0.f;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        x[i] = live ? __bfloat162float(xq[k][i]) : 0.f;
+      for (int i = 0; i < QV; ++i) {
+        const uint32_t w = live ? xq[k][i / 2] : 0u;
+        x[i] = __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
         m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
       }
       m = warp_max(m);
       const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
-      const float s = bad ? 1.f : kv8_scale(m), rs = 1.f / s;  // powers of two
+      const float s = bad ? 1.f : kv8_scale(m);
+      const float rs = bad ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, powers of two
+      uint32_t hi = 0u, lo = 0u;  // the lane's codes
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const int e = lane + 32 * i;
-        const float y = bad ? 0.f : x[i] * rs;
-        const uint32_t hi = e4m3x2(y, 0.f);
-        const uint32_t lo = e4m3x2(y - e4m3x2_value(hi).x, 0.f);
-        uint8_t* dst = smem + T::OFF_Q + (e / 16) * (T::NS * 16) + e % 16;
-        dst[c * 16] = (uint8_t)hi;
-        dst[(RT + c) * 16] = (uint8_t)lo;
+      for (int i = 0; i < QV; i += 2) {
+        const float y0 = bad ? 0.f : x[i] * rs, y1 = bad ? 0.f : x[i + 1] * rs;
+        const uint32_t h2 = e4m3x2(y0, y1);
+        const float2 v = e4m3x2_value(h2);
+        hi |= h2 << (8 * i);
+        lo |= e4m3x2(y0 - v.x, y1 - v.y) << (8 * i);
       }
-      if (lane == 0) {
-        qf[c] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
-        for (int g = 0; g < NTG; ++g) {
-          refs[g * RT + c] = 0.f;
-          haves[g * RT + c] = 0.f;
-        }
-        // a column without a query sees whatever there is; its output is zero, or none
-        qhi[c] = live ? min(shift + t, k1 - 1) : k1 - 1;
-        outs[c] = t >= a.seq ? -1 : (((int64_t)b * a.seq + t) * a.ldo + (int64_t)h * HD) * 2 + (live ? 1 : 0);
-        if (ALIBI) slope[c] = exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * kLog2e;
+      uint8_t* dst = smem + T::OFF_Q + (lane * QV / 16) * (T::NS * 16) + lane * QV % 16;
+      if constexpr (QV == 4) {
+        *reinterpret_cast<uint32_t*>(dst + c * 16) = hi;
+        *reinterpret_cast<uint32_t*>(dst + (RT + c) * 16) = lo;
+      } else {
+        *reinterpret_cast<uint16_t*>(dst + c * 16) = (uint16_t)hi;
+        *reinterpret_cast<uint16_t*>(dst + (RT + c) * 16) = (uint16_t)lo;
       }
+      if (lane == 0) qf[c] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
     }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
-    soft_sync<kSoftWarps>();
+    cols_sync<kSoftWarps + 1>();
 
     // ------------------------------------------------------------------ softmax
     const int wg = warp >> 2, w4 = warp & 3, tg = wg / NCG, c0 = (wg % NCG) * CPW;
@@ -565,9 +601,9 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
       // y of this key for the group's columns: z + bias - ref (ref = bias before the first)
       float y[CPW];
       {
-        uint32_t hi[CPW], lo[CPW];
-        tmem_ld<CPW>(tl + (i & 1) * T::NS + c0, hi);
-        tmem_ld<CPW>(tl + (i & 1) * T::NS + RT + c0, lo);
+        uint32_t hi[CPW], lo[T::SUM ? 1 : CPW];
+        tmem_ld<CPW>(tl + (i & 1) * T::SC + c0, hi);
+        if constexpr (!T::SUM) tmem_ld<CPW>(tl + (i & 1) * T::SC + RT + c0, lo);
         tmem_ld_wait();
         const uint64_t ks2 = f2pack(ks, ks), ev2 = f2pack(ev, ev);
 #pragma unroll
@@ -576,8 +612,8 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
           const uint64_t f2[2] = {f2pack(f4.x, f4.y), f2pack(f4.z, f4.w)}, r2[2] = {f2pack(r4.x, r4.y), f2pack(r4.z, r4.w)};
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
-            const uint64_t s2 = fadd2(f2pack(__uint_as_float(hi[c + e]), __uint_as_float(hi[c + e + 1])),
-                                      f2pack(__uint_as_float(lo[c + e]), __uint_as_float(lo[c + e + 1])));
+            uint64_t s2 = f2pack(__uint_as_float(hi[c + e]), __uint_as_float(hi[c + e + 1]));
+            if constexpr (!T::SUM) s2 = fadd2(s2, f2pack(__uint_as_float(lo[c + e]), __uint_as_float(lo[c + e + 1])));
             f2unpack(ffma2(s2, fmul2(ks2, f2[e / 2]), fadd2(ev2, r2[e / 2])), y[c + e], y[c + e + 1]);
           }
         }
@@ -750,14 +786,21 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     }
     refs[c] = r;
     lsum[c] = den;
+    if (splits == 1) {  // nothing to join: the factors normalise
+      const float inv = 1.f / den;
+      facs[c] *= inv;
+      if (NTG == 2) facs[RT + c] *= inv;
+      if (den == 0.f) outs[c] &= ~1ll;  // a column that saw nothing
+    }
   }
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
   if (splits > 1) cluster_wait();  // every CTA of the cluster has started
   __syncthreads();
   const int piece = RT * HD / splits, cols = max(1, piece / HD);  // of one owner (powers of two)
   const int lp = 31 - __clz(piece), lc = 31 - __clz(cols);
   const float* in = reinterpret_cast<const float*>(smem + T::OFF_IN);
   const float2* inl = reinterpret_cast<const float2*>(smem + T::OFF_INL);
-  if ((int)threadIdx.x < splits * cols) {
+  if (splits > 1 && (int)threadIdx.x < splits * cols) {
     const int to = (int)threadIdx.x >> lc, k = (int)threadIdx.x & (cols - 1), c = (to << lp) / HD + k;
     st_peer2(peer_addr(inl + split * cols + k, to), refs[c], lsum[c]);
   }
@@ -771,16 +814,27 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = 0.f;
+      __syncwarp();
 #pragma unroll 1
-      for (int x = 0; x < 3 * min(NTG, tiles); ++x) {  // group x / 3, term x % 3
-        const float unit = x % 3 == 0 ? 1.f : x % 3 == 1 ? 0.125f : 0.015625f;
-        uint32_t v[8];
-        tmem_ld<8>(tl + (x / 3) * T::NO + (x % 3) * RT + c, v);
+      for (int g = 0; g < min(NTG, tiles); ++g) {
+        uint32_t v[3][8];
+#pragma unroll
+        for (int term = 0; term < 3; ++term) tmem_ld<8>(tl + g * T::NO + term * RT + c, v[term]);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(facs[(x / 3) * RT + c + e] * unit, __uint_as_float(v[e]), o[e]);
+        for (int e = 0; e < 8; ++e) {
+          const float sum = fmaf(0.015625f, __uint_as_float(v[2][e]), fmaf(0.125f, __uint_as_float(v[1][e]), __uint_as_float(v[0][e])));
+          o[e] = fmaf(facs[g * RT + c + e], sum, o[e]);
+        }
       }
-      if (HD == 128 || lane < 16) {
+      const bool own = HD == 128 || lane < 16;
+      if (splits == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int64_t to = outs[c + e];
+          if (own && ok && to >= 0) out[(to >> 1) + dim] = __float2bfloat16_rn(to & 1 ? o[e] : 0.f);
+        }
+      } else if (own) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int idx = (c + e) * HD + dim;
@@ -793,21 +847,38 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   if (splits > 1) cluster_sync();
   else __syncthreads();
   if (warp == kSoftWarps) tmem_dealloc(tmem, T::TMEM);
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
+  if (splits == 1) return;
   const int first = split * piece / HD;
-  for (int idx = threadIdx.x; ok && idx < piece; idx += T::THREADS) {
+  for (int idx = (int)threadIdx.x * 4; ok && idx < piece; idx += T::THREADS * 4) {
     const int e = split * piece + idx, c = e / HD;
     const int64_t to = outs[c];
     if (to < 0) break;
-    float ref = kNoRef, num = 0.f, den = 0.f;
-    for (int s = 0; s < splits; ++s) ref = fminf(ref, inl[s * cols + c - first].x);
+    const float2* rl = inl + c - first;  // the splits' references and sums
+    float ref = kNoRef, den = 0.f, v[4] = {};
+    for (int s = 0; s < splits; ++s) ref = fminf(ref, rl[s * cols].x);
     for (int s = 0; s < splits; ++s) {
-      const float2 rl = inl[s * cols + c - first];
-      const float f = fast_exp2(ref - rl.x);
-      num = fmaf(f, in[s * piece + idx], num);
-      den = fmaf(f, rl.y, den);
+      const float2 w = rl[s * cols];
+      const float4 x = *reinterpret_cast<const float4*>(in + s * piece + idx);
+      const float f = fast_exp2(ref - w.x);
+      den = fmaf(f, w.y, den);
+      v[0] = fmaf(f, x.x, v[0]);
+      v[1] = fmaf(f, x.y, v[1]);
+      v[2] = fmaf(f, x.z, v[2]);
+      v[3] = fmaf(f, x.w, v[3]);
     }
-    out[(to >> 1) + e % HD] = __float2bfloat16_rn((to & 1) && den != 0.f ? num / den : 0.f);
+    const float inv = 1.f / den;
+    uint2 codes = make_uint2(0u, 0u);
+    if ((to & 1) && den != 0.f) codes = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+    __nv_bfloat16* dst = out + (to >> 1) + e % HD;
+    if (reinterpret_cast<uintptr_t>(dst) % 8 == 0) {
+      *reinterpret_cast<uint2*>(dst) = codes;
+    } else {
+      uint16_t* d = reinterpret_cast<uint16_t*>(dst);
+      d[0] = (uint16_t)codes.x;
+      d[1] = (uint16_t)(codes.x >> 16);
+      d[2] = (uint16_t)codes.y;
+      d[3] = (uint16_t)(codes.y >> 16);
+    }
   }
 }
 
