@@ -35,7 +35,9 @@ WV_DEV float block_max(float v, float* tmp) {
 // ------------------------------------------------------------------- append
 // One CTA per (block of a sequence, KV head, K or V): any even head_dim and stride.
 // Rotated keys are computed twice (once for the maximum), with the products and the
-// sum rounded one by one so that a key is the same code on every path.
+// sum rounded one by one so that a key is the same code on every path. Bound by the issue
+// of its two-byte accesses: 476 us for 4 x 4096 tokens of 32 heads of 128 (73 us below),
+// 3.5 us for one token each of 64 sequences (2.8).
 __global__ void __launch_bounds__(128) kv8_append_kernel(const Kv8AppendArgs a) {
   pdl_wait();
   pdl_trigger();
@@ -261,7 +263,9 @@ constexpr int kGenWarps = 4;
 
 // One CTA per (query row, head): warp w takes the 32-key groups w, w + 4, ... of the
 // row's keys, a lane per key for the scores and a lane per dimension for the values,
-// with a running maximum and sum; the warps merge in shared memory, in warp order.
+// with a running maximum and sum; the warps merge in shared memory, in warp order. Bound
+// by instructions, and a KV head is read once for each of its query heads: 64 x 4096
+// tokens, 32 heads over 8 of 64, take 1605 us (46 on the tensor cores).
 template <bool ALIBI>
 __global__ void __launch_bounds__(kGenWarps * 32) kv8_attn_rows_kernel(const Kv8AttnArgs a) {
   pdl_wait();
