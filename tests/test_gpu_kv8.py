@@ -441,6 +441,52 @@ def test_attention_strides_streams_and_repeatability(torch_cuda):
         assert torch.equal(first, outw)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,kv", [(1, 2), (160, 2), (7, 3)])
+@pytest.mark.parametrize("seq", [1, 9, 40])
+def test_attention_alignment_changes_nothing(torch_cuda, hd, batch, kv, seq):
+    """Rows at any 2-byte address give the bits of aligned ones, with a split context
+    and with more sequences than fit at once."""
+    torch = torch_cuda
+    heads = 2 * kv
+    ctx = [40 + (b * 97) % 461 for b in range(batch)]
+    cache = _cache(torch, batch, ctx, kv, hd, seed=9)
+    cfg = _config(heads, kv, hd)
+    q = torch.randn(batch * seq, heads * hd, device="cuda").bfloat16()
+    out = torch.empty_like(q)
+    W.kv8_attention(cfg, cache, seq, q, out, max(ctx))
+    for off, extra in ((1, 3), (2, 2), (4, 8)):
+        wide = torch.zeros(batch * seq, heads * hd + off + extra, device="cuda", dtype=torch.bfloat16)
+        outw = torch.full_like(wide, 5.0)
+        wide[:, off:off + heads * hd] = q
+        W.kv8_attention(cfg, cache, seq, wide[:, off:off + heads * hd], outw[:, off:off + heads * hd], max(ctx))
+        W.device_check()
+        assert torch.equal(outw[:, off:off + heads * hd], out)
+        assert bool((outw[:, :off] == 5).all()) and bool((outw[:, off + heads * hd:] == 5).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv", [1, 3, 5, 6])
+@pytest.mark.parametrize("rope", [False, True])
+def test_append_alignment_changes_nothing(torch_cuda, hd, kv, rope):
+    """Rows that are not aligned take another kernel and give the same codes and scales,
+    for any number of heads, whether a block is begun, continued or left partial."""
+    torch = torch_cuda
+    batch, seq = 3, 70
+    ctx, lens = [70, 203, 131], [70, 9, 33]
+    table = torch.empty(max(ctx), hd // 2, 2, device="cuda")
+    W.rope_table(max(ctx), hd, table)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    wide = (torch.randn(2, batch * seq, kv * hd + 1, device="cuda") * 3).bfloat16()
+    got = []
+    for k, v in ((wide[0, :, 1:], wide[1, :, 1:]), (wide[0, :, 1:].contiguous(), wide[1, :, 1:].contiguous())):
+        cache = _cache(torch, batch, ctx, kv, hd, seed=4)
+        W.kv8_append(cache, seq, k, v, rope=table if rope else None, seq_lens=sl)
+        W.device_check()
+        got.append(cache.tensors[:4])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_attention_head_shard(torch_cuda):
     """A shard of the heads over its own KV heads equals those heads of the whole,
     ALiBi slopes included."""
