@@ -26,8 +26,8 @@
 // scales of a row's blocks may lie 2^100 apart). ref is a column's running maximum of z,
 // raised only when it is exceeded by more than 2^10 (E5M2 has the room), so that after the
 // first tile one vote and no maximum is the rule; when it moves, O and l are rescaled.
-// (Room of 2^3 and remainders that need no factor of 8 are 16 instructions fewer of 400
-// but move references more often: 625 us against 574 for the prompt piece below.)
+// (Room of 2^3 and remainders that need no factor of 8 are 16 instructions fewer
+// but move references more often: 625 us against 574, at the time, for the prompt piece below.)
 //
 // Roles: softmax warpgroups (thread = TMEM lane = key; each takes CPW of the columns), a
 // TMA warp (pages of codes and their four scales into rings of 128-key tiles), an MMA
@@ -43,9 +43,9 @@
 // codes and scales; 64 of 4096, 8 KV heads of 64 for 32 heads: 46 us, 5.3 TB/s; 5 tokens
 // each for 8 sequences in a window of 8192, 8 KV heads of 128: 34-38 us, 3.6-4 TB/s (6.3
 // in the loop, the rest is the first tile's chain of lengths, page ids, copies, MMA and
-// softmax, and the joining); 2048 tokens over 10001, 32 heads of 128: 563 us, 535
+// softmax, and the joining); 2048 tokens over 10001, 32 heads of 128: 556 us, 542
 // TFLOP/s. The first three are bound by HBM; the last by the issue of the softmax, about
-// 400 instructions a warp and tile of 16 columns (the tensor pipe is 30 % busy).
+// 290 instructions a warp and tile of 16 columns (the tensor pipe is 30 % busy).
 // Masked keys and rows past the context: their p is set to 0 and their V rows cleared
 // (a byte never written may be a NaN code); NaN scales reach only columns that see them.
 #include "attn_common.cuh"
@@ -206,7 +206,8 @@ template <int ID> WV_DEV bool bar_any(bool v) {
   return r != 0;
 }
 template <int ID> WV_DEV void bar_sync() { asm volatile("barrier.cta.sync %0, 128;" ::"n"(ID) : "memory"); }
-// ... of warpgroup w of N (barrier 0 is the CTA's).
+// ... of warpgroup w of N (barrier 0 is the CTA's; numbers known to the compiler, since a
+// barrier by register made the prompt piece above take 563 us instead of 557).
 template <int N> WV_DEV bool wg_any(int w, bool v) {
   if (N == 1 || w == 0) return bar_any<1>(v);
   if (N == 2 || w == 1) return bar_any<2>(v);
@@ -579,11 +580,14 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     for (int c = 0; c < CPW / 2; ++c) l2[c] = 0ull;
     int slot = 0;  // of the scales' ring, and its pass
     uint32_t pass = 0;
+    // Tiles up to low_edge (a window) and from high_edge on hold some column's edge.
+    const int low_edge = a.window > 0 && k1 - 1 - a.window >= base0 ? (k1 - 1 - a.window - base0) / kKeys : -1;
+    const int high_edge = qlo + 1 >= base0 + kKeys ? (qlo + 1 - base0) / kKeys : 0;
     for (int i = 0; i < tiles; ++i) {
-      const int base = base0 + i * kKeys, kpos = base + key;
+      const int kpos = base0 + i * kKeys + key;
       // After a wait that gave up, the tiles are still walked (the waits return at once):
       // the warpgroup's barriers need every thread.
-      ok = mbar_wait(&sc_full[slot], pass, abort_flag, a.err, kErrWaitFull) && ok;
+      mbar_wait(&sc_full[slot], pass, abort_flag, a.err, kErrWaitFull);
       const uint32_t sc = sm + T::OFF_SC + slot * 64 + (key >> 4) * 4;
       if (++slot == T::SCALES) {
         slot = 0;
@@ -593,15 +597,19 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
       const float ks = lds(sc), vs = lds(sc + 32);
       float ev;
       asm("lg2.approx.f32 %0, %1;" : "=f"(ev) : "f"(vs));
-      const float inv = on && vs == vs ? __fdividef(1.f, vs) : 0.f;
-      ok = mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull) && ok;
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(vs));
+      if (!on || vs != vs) inv = 0.f;
+      mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccFull);
       // Rows past the context may hold NaN codes, and 0 * NaN is NaN: cleared, now that
       // S_i has come and PV_{i-2}, the last reader of an earlier tile in this slot, is done.
-      if (!on && c0 == 0) {
-        ok = mbar_wait(&v_full[i % VST], (i / VST) & 1, abort_flag, a.err, kErrWaitFull) && ok;
-        const uint32_t row = sm + T::OFF_V + (i % VST) * T::TILE + key * HD;
+      if (base0 + (i + 1) * kKeys > k1 && c0 == 0) {
+        mbar_wait(&v_full[i % VST], (i / VST) & 1, abort_flag, a.err, kErrWaitFull);
+        if (!on) {
+          const uint32_t row = sm + T::OFF_V + (i % VST) * T::TILE + key * HD;
 #pragma unroll 1
-        for (int x = 0; x < HD; x += 16) sts4(row + x, 0u, 0u, 0u, 0u);
+          for (int x = 0; x < HD; x += 16) sts4(row + x, 0u, 0u, 0u, 0u);
+        }
       }
       __syncwarp();  // lanes leave a wait one by one; the TMEM loads need them together
       tc_fence_after();
@@ -629,8 +637,7 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
 #pragma unroll
         for (int c = 0; c < CPW; ++c) y[c] -= slope[c0 + c] * (float)(qhi[c0 + c] - kpos);
       }
-      // some column's edge lies in the tile
-      if (base + kKeys > qlo + 1 || (a.window > 0 && base <= k1 - 1 - a.window)) {
+      if (i >= high_edge || i <= low_edge) {
         const int w = a.window > 0 ? a.window : INT_MAX;
 #pragma unroll
         for (int c = 0; c < CPW; ++c) {
@@ -657,8 +664,7 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
             if (lane == 0) sts(red + (w4 * RT + c + e) * 4, m);
           }
         }
-        if (i > 0)
-          ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+        if (i > 0) mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty);
         __syncwarp();
         tc_fence_after();
         wg_sync<NCG>(wg);
@@ -767,7 +773,8 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     }
     // every PV has completed (the last two cover the others: MMAs finish in order)
     for (int i = max(0, tiles - 2); i < tiles; ++i)
-      ok = mbar_wait(&pv_done[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty) && ok;
+      mbar_wait(&pv_done[i & 1], (i >> 1) & 1, abort_flag, a.err, kErrWaitAccEmpty);
+    ok = *abort_flag == 0;  // a wait that gave up has set it
     tc_fence_after();
   }
   // A bounded wait that gave up is in the error word: every thread still takes the
