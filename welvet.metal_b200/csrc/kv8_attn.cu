@@ -45,7 +45,7 @@
 // in the loop, the rest is the first tile's chain of lengths, page ids, copies, MMA and
 // softmax, and the joining); 2048 tokens over 10001, 32 heads of 128: 556 us, 542
 // TFLOP/s. The first three are bound by HBM; the last by the issue of the softmax, about
-// 290 instructions a warp and tile of 16 columns (the tensor pipe is 30 % busy).
+// 300 instructions a warp and tile of 16 columns (the tensor pipe is 30 % busy).
 // Masked keys and rows past the context: their p is set to 0 and their V rows cleared
 // (a byte never written may be a NaN code); NaN scales reach only columns that see them.
 #include "attn_common.cuh"
