@@ -322,35 +322,31 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
   const int split = blockIdx.x % splits, b = blockIdx.z;
   const int kh = blockIdx.y, r0 = (int)(blockIdx.x / splits) * RT;
   const int G = a.heads / a.c.kv_heads;
-  constexpr int NQ = (RT + kSoftWarps - 1) / kSoftWarps;  // columns of a softmax warp
-  constexpr int QV = HD / 32;  // consecutive dims of a lane
-  uint32_t xq[NQ][QV / 2];
-  int tq = 0;  // lane k: the token of the warp's column k
+  // Eight lanes a column, QD dims each: 4 columns a warp.
+  constexpr int QD = HD / 8;
+  static_assert(RT <= kSoftWarps * 4, "columns of the softmax warps");
+  uint32_t xq[QD / 2];
+  const int qc = warp * 4 + lane / 8, qd = lane % 8 * QD;
+  int tq = 0;  // the column's token
   if (warp < kSoftWarps) {
-    const bool wide = (reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.ldq * 2) % (2 * QV) == 0;
-    const int c = warp + lane % NQ * kSoftWarps;
-    tq = (r0 + c) / G;
-    const int64_t at = ((int64_t)b * a.seq + tq) * a.ldq + (int64_t)(kh * G + (r0 + c) - tq * G) * HD;
-    const bool there = c < RT && tq < a.seq;
+    tq = (r0 + qc) / G;
+    const uint16_t* x = static_cast<const uint16_t*>(a.q) + ((int64_t)b * a.seq + tq) * a.ldq +
+                        (int64_t)(kh * G + (r0 + qc) - tq * G) * HD + qd;
 #pragma unroll
-    for (int k = 0; k < NQ; ++k) {
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + __shfl_sync(0xffffffffu, at, k);
-      const uint16_t* x = reinterpret_cast<const uint16_t*>(q) + lane * QV;
+    for (int i = 0; i < QD / 2; ++i) xq[i] = 0u;
+    if (qc < RT && tq < a.seq) {
+      if (reinterpret_cast<uintptr_t>(x) % 16 == 0) {
 #pragma unroll
-      for (int i = 0; i < QV / 2; ++i) xq[k][i] = 0u;
-      if (__shfl_sync(0xffffffffu, there, k)) {
-        if (wide) {
-          if constexpr (QV == 4) {
-            const uint2 v = *reinterpret_cast<const uint2*>(x);
-            xq[k][0] = v.x;
-            xq[k][1] = v.y;
-          } else {
-            xq[k][0] = *reinterpret_cast<const uint32_t*>(x);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < QV / 2; ++i) xq[k][i] = x[2 * i] | (uint32_t)x[2 * i + 1] << 16;
+        for (int i = 0; i < QD / 2; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(x + 2 * i);
+          xq[i] = v.x;
+          xq[i + 1] = v.y;
+          xq[i + 2] = v.z;
+          xq[i + 3] = v.w;
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < QD / 2; ++i) xq[i] = x[2 * i] | (uint32_t)x[2 * i + 1] << 16;
       }
     }
   }
@@ -525,41 +521,40 @@ __global__ void __launch_bounds__(KT<HD, RT>::THREADS, KT<HD, RT>::PER_SM)
     }
   } else {
     // ---- queries: hi and lo codes, [16-byte chunk of hd][RT hi rows, RT lo rows][16]
+    const bool live = tq >= t0 && tq <= t1;
+    float m = 0.f;
 #pragma unroll
-    for (int k = 0; k < NQ; ++k) {
-      const int c = warp + k * kSoftWarps;
-      if (c >= RT) break;
-      const int t = __shfl_sync(0xffffffffu, tq, k);
-      const bool live = t >= t0 && t <= t1;
-      float x[QV], m = 0.f;
+    for (int i = 0; i < QD; ++i) {
+      if (!live) xq[i / 2] = 0u;
+      const float x = __uint_as_float(i & 1 ? xq[i / 2] & 0xffff0000u : xq[i / 2] << 16);
+      m = fmaxf(m, x - x == 0.f ? fabsf(x) : INFINITY);
+    }
 #pragma unroll
-      for (int i = 0; i < QV; ++i) {
-        const uint32_t w = live ? xq[k][i / 2] : 0u;
-        x[i] = __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-        m = fmaxf(m, x[i] - x[i] == 0.f ? fabsf(x[i]) : INFINITY);
-      }
-      m = warp_max(m);
-      const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
-      const float s = bad ? 1.f : kv8_scale(m);
-      const float rs = bad ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, powers of two
-      uint32_t hi = 0u, lo = 0u;  // the lane's codes
+    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool bad = m == INFINITY;  // a query that is not finite: its column is NaN
+    const float s = bad ? 1.f : kv8_scale(m);
+    const float rs = bad ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, powers of two
+    uint32_t hi[QD / 4], lo[QD / 4];  // the lane's codes
 #pragma unroll
-      for (int i = 0; i < QV; i += 2) {
-        const float y0 = bad ? 0.f : x[i] * rs, y1 = bad ? 0.f : x[i + 1] * rs;
-        const uint32_t h2 = e4m3x2(y0, y1);
-        const float2 v = e4m3x2_value(h2);
-        hi |= h2 << (8 * i);
-        lo |= e4m3x2(y0 - v.x, y1 - v.y) << (8 * i);
-      }
-      uint8_t* dst = smem + T::OFF_Q + (lane * QV / 16) * (T::NS * 16) + lane * QV % 16;
-      if constexpr (QV == 4) {
-        *reinterpret_cast<uint32_t*>(dst + c * 16) = hi;
-        *reinterpret_cast<uint32_t*>(dst + (RT + c) * 16) = lo;
+    for (int i = 0; i < QD; i += 2) {
+      const float x0 = __uint_as_float(xq[i / 2] << 16), x1 = __uint_as_float(xq[i / 2] & 0xffff0000u);
+      const float y0 = bad ? 0.f : x0 * rs, y1 = bad ? 0.f : x1 * rs;
+      const uint32_t h2 = e4m3x2(y0, y1);
+      const float2 v = e4m3x2_value(h2);
+      const uint32_t l2c = e4m3x2(y0 - v.x, y1 - v.y);
+      hi[i / 4] = i % 4 ? hi[i / 4] | h2 << 16 : h2;
+      lo[i / 4] = i % 4 ? lo[i / 4] | l2c << 16 : l2c;
+    }
+    if (qc < RT) {
+      uint8_t* dst = smem + T::OFF_Q + (qd / 16) * (T::NS * 16) + qd % 16 + qc * 16;
+      if constexpr (QD == 16) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + RT * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       } else {
-        *reinterpret_cast<uint16_t*>(dst + c * 16) = (uint16_t)hi;
-        *reinterpret_cast<uint16_t*>(dst + (RT + c) * 16) = (uint16_t)lo;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(dst + RT * 16) = make_uint2(lo[0], lo[1]);
       }
-      if (lane == 0) qf[c] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
+      if (lane % 8 == 0) qf[qc] = bad ? __uint_as_float(0x7fc00000u) : s * a.scale * kLog2e;
     }
     fence_proxy_async_smem();
     __syncwarp();
