@@ -26,8 +26,8 @@
 // scales of a row's blocks may lie 2^100 apart). ref is a column's running maximum of z,
 // raised only when it is exceeded by more than 2^10 (E5M2 has the room), so that after the
 // first tile one vote and no maximum is the rule; when it moves, O and l are rescaled.
-// (Room of 2^3 and remainders that need no factor of 8 are 16 instructions fewer
-// but move references more often: 625 us against 574, at the time, for the prompt piece below.)
+// (Room of 2^3 and remainders that need no factor of 8 are 16 instructions fewer but move
+// references more often: 625 us against 574, at the time, for the prompt piece below.)
 //
 // Roles: softmax warpgroups (thread = TMEM lane = key; each takes CPW of the columns), a
 // TMA warp (pages of codes and their four scales into rings of 128-key tiles), an MMA
@@ -43,7 +43,7 @@
 // codes and scales; 64 of 4096, 8 KV heads of 64 for 32 heads: 46 us, 5.3 TB/s; 5 tokens
 // each for 8 sequences in a window of 8192, 8 KV heads of 128: 34-38 us, 3.6-4 TB/s (6.3
 // in the loop, the rest is the first tile's chain of lengths, page ids, copies, MMA and
-// softmax, and the joining); 2048 tokens over 10001, 32 heads of 128: 556 us, 542
+// softmax, and the joining); 2048 tokens over 10001, 32 heads of 128: 555 us, 543
 // TFLOP/s. The first three are bound by HBM; the last by the issue of the softmax, about
 // 300 instructions a warp and tile of 16 columns (the tensor pipe is 30 % busy).
 // Masked keys and rows past the context: their p is set to 0 and their V rows cleared
