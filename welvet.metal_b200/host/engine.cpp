@@ -119,6 +119,23 @@ PrimaryCtxStateFn primary_ctx_state_fn() {
   }();
   return fn;
 }
+
+// Whether the calling thread has a context. A thread that has made no CUDA call has
+// none, although cudaGetDevice names a device for it; kernel launches would create it,
+// the encoding of TMA descriptors fails without.
+bool has_context() {
+  using CtxGetCurrentFn = int (*)(void** ctx);
+  static CtxGetCurrentFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<CtxGetCurrentFn>(p);
+    return static_cast<CtxGetCurrentFn>(nullptr);
+  }();
+  void* ctx = nullptr;
+  return fn && fn(&ctx) == 0 && ctx;
+}
 }  // namespace
 
 DeviceRestore::DeviceRestore() {
@@ -176,7 +193,7 @@ Status device_ctx(int device, DeviceCtx** out) {
   auto it = g_devs.find(device);
   if (it != g_devs.end()) {
     *out = it->second;
-    if (current) return Status::ok();  // its context exists, and it is current already
+    if (current && has_context()) return Status::ok();
     return cudaSetDevice(device) == cudaSuccess ? Status::ok() : Status::err(4, "cudaSetDevice");
   }
   WV_CUDA(cudaSetDevice(device), "cudaSetDevice");
