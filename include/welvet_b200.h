@@ -140,7 +140,8 @@ WELVET_API welvet_status welvet_b200_kv_create_e4m3(welvet_b200_mha* layer, int3
 /* seq new tokens per sequence at positions ctx_len[b] ... ctx_len[b] + seq - 1 (a later
  * piece of a prompt, proposed tokens to verify): x_new, post [batch * seq, d_model], row
  * b * seq + t; their keys and values are appended and every row attends over the cache up
- * to its own position. E4M3 caches (code 2 otherwise); seq 1 is mha_decode. */
+ * to its own position. E4M3 caches (code 2 otherwise); seq 1 is mha_decode. A step that
+ * is refused, here or in mha_decode, leaves the lengths as they were. */
 WELVET_API welvet_status welvet_b200_mha_extend(welvet_b200_mha* layer, welvet_b200_kv* kv,
                                                 int32_t batch, int32_t seq, const void* x_new, void* pre,
                                                 void* post, int32_t on_device, void* stream);

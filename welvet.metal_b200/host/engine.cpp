@@ -879,10 +879,10 @@ Status mha_forward(Mha* m, int batch, int seq, const void* x, void* pre, void* p
     if (kv && kv->e4m3) {  // prefill into an E4M3 cache (single chunk)
       WV_CUDA(set_ctx(kv->ctx_len.as<int>(), batch, seq, s), "ctx");
       count_launch();
+      for (int b = 0; b < batch; ++b) kv->ctx_host[b] = seq;
       const char* base = static_cast<const char*>(m->qkv.p);
       WV_TRY(kv8_append_rows(kv, batch, seq, base + (size_t)m->qd_l * es, base + (size_t)(m->qd_l + m->kd_l) * es,
                              m->nqkv, s));
-      for (int b = 0; b < batch; ++b) kv->ctx_host[b] = seq;
     } else if (kv) {  // prefill: K/V rows into the cache pages of each sequence (single chunk)
       WV_TRY(m->slots.ensure(M * 4));
       WV_CUDA(make_prefill_slots(m->slots.as<int>(), batch, seq, kv->pages_per_seq, s), "slots");
@@ -1263,8 +1263,8 @@ Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on
     if (kv->e4m3) {
       WV_CUDA(set_ctx(kv->ctx_len.as<int>(), batch, ctx, s), "ctx");
       count_launch();
-      WV_TRY(kv8_append_rows(kv, batch, ctx, kd, vd, m->kd_l, s));
       for (int b = 0; b < batch; ++b) kv->ctx_host[b] = ctx;
+      WV_TRY(kv8_append_rows(kv, batch, ctx, kd, vd, m->kd_l, s));
       if (!on_device) WV_CUDA(cudaStreamSynchronize(s), "kv fill");
       return Status::ok();
     }
@@ -1282,15 +1282,13 @@ Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on
   return Status::ok();
 }
 
-Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, void* post, bool on_device,
-                  cudaStream_t s) {
-  if (!m || !kv || kv->layer != m || !x || !post || batch <= 0 || batch > kv->max_batch || seq <= 0 ||
-      (int64_t)batch * seq >= (int64_t{1} << 30))
-    return Status::err(1, "mha decode: invalid argument");
-  if (seq > 1 && !kv->e4m3) return Status::err(2, "mha extend: needs an E4M3 cache");
-  if ((int64_t)seq * m->hc > INT32_MAX) return Status::err(1, "mha extend: seq * heads too large");
+namespace {
+
+// The step itself. *ahead: the device's lengths count the new tokens, the host's do not
+// yet.
+Status decode_step(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, void* post, bool on_device,
+                   cudaStream_t s, bool* ahead) {
   const int rows = batch * seq;
-  std::lock_guard<std::mutex> lock(m->mu);
   WV_CUDA(cudaSetDevice(m->dev->device), "cudaSetDevice");
   const auto& c = m->cfg;
   const int dm = c.c.d_model;
@@ -1312,6 +1310,7 @@ Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, 
   }
   WV_TRY(m->positions.ensure((size_t)rows * 4));
   WV_TRY(m->slots.ensure((size_t)batch * 4));
+  *ahead = true;
   if (kv->e4m3) {
     WV_CUDA(make_extend_rows(kv->ctx_len.as<int>(), m->positions.as<int>(), batch, seq, s), "decode rows");
   } else {
@@ -1458,6 +1457,7 @@ Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, 
     prof_end(kProfAllReduce, s);
   }
   for (int b = 0; b < batch; ++b) kv->ctx_host[b] += seq;
+  *ahead = false;
   if (!on_device) {
     // pageable outputs with a communicator: copy only after the bounded wait (see
     // mha_forward)
@@ -1469,6 +1469,24 @@ Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, 
     WV_TRY(check_device_error(m->dev));
   }
   return Status::ok();
+}
+
+}  // namespace
+
+Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, void* post, bool on_device,
+                  cudaStream_t s) {
+  if (!m || !kv || kv->layer != m || !x || !post || batch <= 0 || batch > kv->max_batch || seq <= 0 ||
+      (int64_t)batch * seq >= (int64_t{1} << 30))
+    return Status::err(1, "mha decode: invalid argument");
+  if (seq > 1 && !kv->e4m3) return Status::err(2, "mha extend: needs an E4M3 cache");
+  if ((int64_t)seq * m->hc > INT32_MAX) return Status::err(1, "mha extend: seq * heads too large");
+  std::lock_guard<std::mutex> lock(m->mu);
+  bool ahead = false;
+  Status st = decode_step(m, kv, batch, seq, x, pre, post, on_device, s, &ahead);
+  // A step that failed behind the kernel that advances the lengths takes them back.
+  if (!st && ahead)
+    cudaMemcpyAsync(kv->ctx_len.p, kv->ctx_host.data(), (size_t)batch * 4, cudaMemcpyHostToDevice, s);
+  return st;
 }
 
 } // namespace wv
