@@ -1,4 +1,5 @@
-"""KV caches between the steps: a step that is refused leaves the lengths as they were."""
+"""KV caches between the steps: a step that is refused leaves the lengths as they were, and
+an allocation that failed is not reported again by the next call."""
 import pytest
 
 import welvet_b200 as W
@@ -42,3 +43,16 @@ def test_a_refused_step_leaves_the_cache(torch_cuda, e4m3, seq):
         layer.check_device()
         got.append(rows)
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_a_failed_allocation_is_reported_once(torch_cuda):
+    torch = torch_cuda
+    layer = _layer()
+    cache = W.KvCache(layer, 2, 100)
+    with pytest.raises(W.WelvetError) as e:
+        W.KvCache(layer, 400, 1 << 22)  # 2 x 429 GB
+    assert e.value.code == 4 and "memory" in e.value.message
+    cache.fill(2, 0)
+    x = torch.randn(2, 256, device="cuda").bfloat16()
+    layer.decode(cache, 2, x, None, torch.empty_like(x))
+    layer.check_device()

@@ -103,6 +103,7 @@ welvet_status to_c(const Status& s) {
 }
 
 Status cuda_status(cudaError_t e, const char* what) {
+  cudaGetLastError();  // reported here: the next launch must not find it again
   return Status::err(4, std::string("cuda: ") + what + ": " + cudaGetErrorString(e));
 }
 
