@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -240,9 +241,25 @@ def _dtype_name(dtype) -> str:
     return name
 
 
-def _rows(t, rows, width, dtype):
-    """(pointer, row stride) of a 2-D device tensor of `dtype` with at least `rows` rows of
-    `width` values, the values of a row next to each other."""
+def _home(at, device=-1):
+    """Device number `at` of a call's first tensor, which has to be the call's device:
+    `device`, the current one when negative. A host tensor's number is -1."""
+    runs = device if device >= 0 or at < 0 else sys.modules["torch"].cuda.current_device()
+    if at != runs or at < 0:
+        _elsewhere(at, runs)
+    return at
+
+
+def _elsewhere(at, home):
+    name = [f"cuda:{n}" if n >= 0 else "the host" for n in (at, home)]
+    raise ValueError(f"a tensor on {name[0]} in a call that runs on {name[1] if home >= 0 else 'a GPU'}")
+
+
+def _rows(t, rows, width, dtype, home):
+    """(pointer, row stride) of a 2-D tensor of `dtype` on device `home` with at least
+    `rows` rows of `width` values, the values of a row next to each other."""
+    if t.get_device() != home:
+        _elsewhere(t.get_device(), home)
     n, cols = t.shape
     ld, step = t.stride()
     if n < rows or cols < width or t.dtype != dtype or (step != 1 and cols > 1):
@@ -561,35 +578,39 @@ def attention_tf32(cfg: MhaConfig, batch, seq, q, q_lo, k, k_lo, v, v_lo, out, o
 
 def rope_table(max_pos, head_dim, table, theta=10000.0, stream=None):
     """(cos, sin) of pos / theta^(2i/head_dim) into table [max_pos, head_dim/2, 2] FP32."""
-    check(lib().welvet_b200_rope_table(max_pos, head_dim, theta, _typed(table, "float32", max_pos * head_dim),
-                                       _stream(stream)))
+    check(lib().welvet_b200_rope_table(max_pos, head_dim, theta,
+                                       _typed(table, "float32", max_pos * head_dim, _home(table.get_device())), _stream(stream)))
 
 
-def _typed(t, dtype, numel=0):
-    """Device pointer of a contiguous tensor of the given dtype and at least numel values."""
+def _typed(t, dtype, numel, home):
+    """Pointer of a contiguous tensor of the given dtype and at least numel values on
+    device `home`; None for None."""
     if t is None:
         return None
+    if t.get_device() != home:
+        _elsewhere(t.get_device(), home)
     if (_DTYPE_NAMES.get(t.dtype) or _dtype_name(t.dtype)) != dtype or t.numel() < numel or not t.is_contiguous():
         raise ValueError(f"contiguous {dtype} of at least {numel} values expected, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _norm_call(q, k, pairs, head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod):
-    """(io_bf16, arguments) of a norm call up to the row pointers; `pairs` are (queries,
-    keys) tensors with the tokens, widths and dtype of q and k."""
+    """(device, io_bf16, arguments) of a norm call up to the row pointers; `pairs` are
+    (queries, keys) tensors with the tokens, widths and dtype of q and k."""
+    home = _home(q.get_device())
     tokens, qd = q.shape
     kd = 0 if k is None else k.shape[1]
     dtype = q.dtype
     io = 1 if _dtype_name(dtype) == "bfloat16" else 0
     if (not io and _dtype_name(dtype) != "float32") or head_dim <= 0 or qd % head_dim or kd % head_dim:
         raise ValueError("BF16 or FP32 rows of whole heads expected")
-    args = [tokens, qd // head_dim, kd // head_dim, head_dim, eps, _typed(q_gamma, "float32", head_dim),
-            _typed(k_gamma, "float32", head_dim), _typed(rope, "float32"),
-            0 if rope is None else rope.numel() // head_dim, _typed(positions, "int32", tokens), pos_mod]
+    args = [tokens, qd // head_dim, kd // head_dim, head_dim, eps, _typed(q_gamma, "float32", head_dim, home),
+            _typed(k_gamma, "float32", head_dim, home), _typed(rope, "float32", 0, home),
+            0 if rope is None else rope.numel() // head_dim, _typed(positions, "int32", tokens, home), pos_mod]
     for a, b in ((q, k),) + pairs:
-        args += _rows(a, tokens, qd, dtype)
-        args += _rows(b, tokens, kd, dtype) if kd else (None, 0)
-    return io, args
+        args += _rows(a, tokens, qd, dtype, home)
+        args += _rows(b, tokens, kd, dtype, home) if kd else (None, 0)
+    return home, io, args
 
 
 def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1e-6, rope=None, positions=None,
@@ -597,7 +618,7 @@ def qk_norm_rope(q, k, q_out, k_out, head_dim, q_gamma=None, k_gamma=None, eps=1
     """RMS norm of every query and key head with the rotation in the same pass
     (welvet_b200_qk_norm_rope_forward): rows [tokens, heads * head_dim] (may be views of
     one packed row; k may be None), outputs may be the inputs."""
-    io, args = _norm_call(q, k, ((q_out, k_out),), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    _, io, args = _norm_call(q, k, ((q_out, k_out),), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
     check(lib().welvet_b200_qk_norm_rope_forward(*args, io, _stream(stream)))
 
 
@@ -611,12 +632,14 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, dq_gamma, dk_gamma, head
     """Gradient of qk_norm_rope (welvet_b200_qk_norm_rope_backward): dq, dk from the
     forward's inputs and the gradients of its outputs, dq_gamma / dk_gamma [head_dim]
     overwritten with the sums over all rows."""
-    io, args = _norm_call(q, k, ((dq_out, dk_out), (dq, dk)), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    home, io, args = _norm_call(q, k, ((dq_out, dk_out), (dq, dk)), head_dim, q_gamma, k_gamma, eps, rope, positions, pos_mod)
+    if workspace.get_device() != home:
+        _elsewhere(workspace.get_device(), home)
     if workspace.numel() * workspace.element_size() < qk_norm_rope_workspace(head_dim):
         raise ValueError("workspace smaller than qk_norm_rope_workspace(head_dim)")
-    check(lib().welvet_b200_qk_norm_rope_backward(*args, _typed(dq_gamma, "float32", head_dim),
-                                                  _typed(dk_gamma, "float32", head_dim), _ptr(workspace), io,
-                                                  _stream(stream)))
+    check(lib().welvet_b200_qk_norm_rope_backward(*args, _typed(dq_gamma, "float32", head_dim, home),
+                                                  _typed(dk_gamma, "float32", head_dim, home),
+                                                  _ptr(workspace), io, _stream(stream)))
 
 
 class Kv8Cache:
@@ -632,11 +655,14 @@ class Kv8Cache:
             raise ValueError("codes [pages, kv_heads, 64, head_dim] of one byte expected")
         batch, max_pages = block_table.shape
         n = pages * kv_heads * (self.PAGE // self.BLOCK)
+        home = k.get_device()
+        if home < 0 or v.get_device() != home:
+            _elsewhere(v.get_device(), home)
         self.tensors = (k, v, k_scale, v_scale, block_table, ctx_len)
-        self.batch, self.head_dim, self.width = batch, head_dim, kv_heads * head_dim
-        self.args = _Kv8CacheArgs(_ptr(k), _ptr(v), _typed(k_scale, "float32", n),
-                                  _typed(v_scale, "float32", n), _typed(block_table, "int32"),
-                                  _typed(ctx_len, "int32", batch), batch, pages, max_pages, kv_heads, head_dim)
+        self.batch, self.head_dim, self.width, self.device = batch, head_dim, kv_heads * head_dim, home
+        self.args = _Kv8CacheArgs(_ptr(k), _ptr(v), _typed(k_scale, "float32", n, home),
+                                  _typed(v_scale, "float32", n, home), _typed(block_table, "int32", 0, home),
+                                  _typed(ctx_len, "int32", batch, home), batch, pages, max_pages, kv_heads, head_dim)
         self.ref = C.byref(self.args)
 
 
@@ -650,19 +676,21 @@ def _bf16(t):
 def kv8_append(cache: Kv8Cache, seq, k, v, rope=None, seq_lens=None, stream=None):
     """Appends rows b * seq + t of k and v (BF16 [batch * seq, kv_heads * head_dim], may be
     views of packed rows) to the cache (welvet_b200_kv8_append)."""
-    dtype, rows, width = _bf16(k), cache.batch * seq, cache.width
-    check(lib().welvet_b200_kv8_append(cache.ref, seq, _typed(seq_lens, "int32", cache.batch),
-                                       *_rows(k, rows, width, dtype), *_rows(v, rows, width, dtype),
-                                       _typed(rope, "float32"), 0 if rope is None else rope.numel() // cache.head_dim,
-                                       _stream(stream)))
+    dtype, rows, width, home = _bf16(k), cache.batch * seq, cache.width, _home(cache.device)
+    check(lib().welvet_b200_kv8_append(cache.ref, seq, _typed(seq_lens, "int32", cache.batch, home),
+                                       *_rows(k, rows, width, dtype, home), *_rows(v, rows, width, dtype, home),
+                                       _typed(rope, "float32", 0, home),
+                                       0 if rope is None else rope.numel() // cache.head_dim, _stream(stream)))
 
 
 def kv8_attention(cfg: MhaConfig, cache: Kv8Cache, seq, q, out, max_ctx, seq_lens=None, stream=None):
     """Attention of the new tokens (BF16 rows b * seq + t of q) over the cache
     (welvet_b200_kv8_attention)."""
     dtype, rows, width = _bf16(q), cache.batch * seq, (cfg.head_count or cfg.num_heads) * cache.head_dim
-    check(lib().welvet_b200_kv8_attention(C.byref(cfg), cache.ref, seq, _typed(seq_lens, "int32", cache.batch), max_ctx,
-                                          *_rows(q, rows, width, dtype), *_rows(out, rows, width, dtype),
+    home = _home(cache.device, cfg.device)
+    check(lib().welvet_b200_kv8_attention(C.byref(cfg), cache.ref, seq,
+                                          _typed(seq_lens, "int32", cache.batch, home), max_ctx,
+                                          *_rows(q, rows, width, dtype, home), *_rows(out, rows, width, dtype, home),
                                           _stream(stream)))
 
 
