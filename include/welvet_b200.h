@@ -117,6 +117,13 @@ WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 WELVET_API welvet_status welvet_b200_kv_fill(welvet_b200_kv* kv, int32_t batch, int32_t ctx_len,
                                              const void* k, const void* v, int32_t on_device,
                                              void* stream);
+/* Sets the cached length of sequence b to lengths[b] (host array [batch], read before the
+ * call returns; 0 ... max_ctx each), for sequences that keep different numbers of their
+ * last tokens. The next step continues there. In an E4M3 cache a block of 16 tokens that
+ * is cut in the middle keeps the scale that its dropped tokens gave it, NaN included, and
+ * the tokens before the cut keep the codes at that scale, until the block is begun anew. */
+WELVET_API welvet_status welvet_b200_kv_set_lengths(welvet_b200_kv* kv, int32_t batch,
+                                                    const int32_t* lengths, void* stream);
 /* Per-sequence prefill: forward of `seq` tokens per sequence (positions 0..seq-1)
  * that also writes their keys/values into the cache (cached length := seq). */
 WELVET_API welvet_status welvet_b200_mha_prefill(welvet_b200_mha* layer, welvet_b200_kv* kv,

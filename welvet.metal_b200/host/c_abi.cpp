@@ -231,6 +231,12 @@ welvet_status welvet_b200_kv_fill(welvet_b200_kv* kv, int32_t batch, int32_t ctx
   return wv::to_c(wv::kv_fill(kv->kv, batch, ctx_len, k, v, on_device != 0, as_stream(stream)));
 }
 
+welvet_status welvet_b200_kv_set_lengths(welvet_b200_kv* kv, int32_t batch, const int32_t* lengths, void* stream) {
+  wv::DeviceRestore restore_device;
+  if (!kv) return wv::to_c(Status::err(1, "kv: invalid argument"));
+  return wv::to_c(wv::kv_set_lengths(kv->kv, batch, lengths, as_stream(stream)));
+}
+
 welvet_status welvet_b200_mha_prefill(welvet_b200_mha* layer, welvet_b200_kv* kv, int32_t batch, int32_t seq,
                                       const void* x, void* pre, void* post, int32_t on_device, void* stream) {
   wv::DeviceRestore restore_device;

@@ -1283,6 +1283,18 @@ Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on
   return Status::ok();
 }
 
+Status kv_set_lengths(Kv* kv, int batch, const int* lengths, cudaStream_t s) {
+  if (!kv || !lengths || batch <= 0 || batch > kv->max_batch) return Status::err(1, "kv lengths: invalid argument");
+  for (int b = 0; b < batch; ++b)
+    if (lengths[b] < 0 || lengths[b] > kv->max_ctx) return Status::err(1, "kv lengths: outside 0 ... max_ctx");
+  std::lock_guard<std::mutex> lock(kv->layer->mu);
+  WV_CUDA(cudaSetDevice(kv->layer->dev->device), "cudaSetDevice");
+  // pageable host memory: the copy has read it when the call returns
+  WV_CUDA(cudaMemcpyAsync(kv->ctx_len.p, lengths, (size_t)batch * 4, cudaMemcpyHostToDevice, s), "kv lengths");
+  for (int b = 0; b < batch; ++b) kv->ctx_host[b] = lengths[b];
+  return Status::ok();
+}
+
 namespace {
 
 // The step itself. *ahead: the device's lengths count the new tokens, the host's do not

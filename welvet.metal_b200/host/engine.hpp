@@ -250,6 +250,7 @@ struct Kv {
 Status kv_create(Mha* m, int max_batch, int max_ctx, bool e4m3, Kv** out);
 Status kv_fill(Kv* kv, int batch, int ctx, const void* k, const void* v, bool on_device,
                cudaStream_t s);
+Status kv_set_lengths(Kv* kv, int batch, const int* lengths, cudaStream_t s);
 // One step of seq new tokens per sequence (seq > 1: E4M3 caches only).
 Status mha_decode(Mha* m, Kv* kv, int batch, int seq, const void* x, void* pre, void* post,
                   bool on_device, cudaStream_t s);

@@ -48,7 +48,7 @@ EXT_SYMBOLS = ("welvet_b200_mha_config_default", "welvet_b200_mha_mount", "welve
                "welvet_b200_attention_tf32", "welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward",
                "welvet_b200_qk_norm_rope_workspace", "welvet_b200_qk_norm_rope_backward", "welvet_b200_kv8_append",
                "welvet_b200_kv8_attention", "welvet_b200_kv_create_e4m3", "welvet_b200_mha_extend",
-               "welvet_b200_mha_set_qk_norm")
+               "welvet_b200_mha_set_qk_norm", "welvet_b200_kv_set_lengths")
 PROFILE_SLOTS = ("gemm_qkv", "attn_prefill", "gemm_o", "attn_decode", "gemm_qkv_decode", "gemm_o_decode",
                  "allreduce", "other", "gemm_gate_up", "gemm_down", "norm", "embedding", "attn_bwd", "gemm_grad")
 
@@ -188,7 +188,8 @@ def lib():
     L.welvet_b200_kv_create_e4m3.argtypes = [_vp, C.c_int32, C.c_int32, C.POINTER(_vp)]
     L.welvet_b200_mha_extend.argtypes = [_vp, _vp, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int32, _vp]
     L.welvet_b200_mha_set_qk_norm.argtypes = [_vp, C.c_double, _vp, _vp, C.c_int32]
-    for name in ("welvet_b200_kv_create_e4m3", "welvet_b200_mha_extend", "welvet_b200_mha_set_qk_norm",
+    L.welvet_b200_kv_set_lengths.argtypes = [_vp, C.c_int32, _vp, _vp]
+    for name in ("welvet_b200_kv_set_lengths", "welvet_b200_kv_create_e4m3", "welvet_b200_mha_extend", "welvet_b200_mha_set_qk_norm",
                  "welvet_b200_rope_table", "welvet_b200_qk_norm_rope_forward", "welvet_b200_qk_norm_rope_backward",
                  "welvet_b200_kv8_append", "welvet_b200_kv8_attention",
                  "welvet_b200_wait_probe", "welvet_b200_mha_set_output_mode", "welvet_b200_attention_tf32",
@@ -534,6 +535,12 @@ class KvCache:
     def fill(self, batch, ctx_len, k=None, v=None, stream=None):
         on = _on_device(k, v) if k is not None else 1
         check(lib().welvet_b200_kv_fill(self._h, batch, ctx_len, _ptr(k), _ptr(v), on, _stream(stream)))
+
+    def set_lengths(self, lengths, stream=None):
+        """Cached length of each of the first len(lengths) sequences, whole numbers on the
+        host (welvet_b200_kv_set_lengths)."""
+        n = [int(x) for x in lengths]
+        check(lib().welvet_b200_kv_set_lengths(self._h, len(n), (C.c_int32 * len(n))(*n), _stream(stream)))
 
     def close(self):
         if self._h:
