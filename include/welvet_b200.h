@@ -375,9 +375,12 @@ WELVET_API welvet_status welvet_b200_kv8_append(const welvet_b200_kv8_cache* cac
  * cfg: num_heads, num_kv_heads, head_dim, scale_override, mask, window, ALiBi (pos 2 or
  * 3), head shard, precision 1; q and out are BF16 rows, ldq / ldo apart. Rows that see
  * nothing (t >= n_b, an empty sequence) are zero. max_ctx bounds ctx_len (it sizes the
- * split of long contexts, not the result's meaning). Probabilities are rounded to a
- * relative 2^-9, and below 2^-19 of the row's largest to 2^-28 of it. Code 2 for sigmoid
- * scores, other masks and FP32 layers. */
+ * split of long contexts, not the result's meaning). Queries are held to 2^-17 of the
+ * row's largest value. Probabilities are rounded to a relative 2^-9, and below 2^-19 of the
+ * row's largest to 2^-28 of it; their sum takes them unrounded. head_dim 64 and 128 with
+ * 16-byte aligned pools run on the tensor cores; the other sizes on a general kernel that
+ * does not split contexts (35 times the time for 64 sequences of 4096 tokens), without
+ * either rounding. Code 2 for sigmoid scores, other masks and FP32 layers. */
 WELVET_API welvet_status welvet_b200_kv8_attention(const welvet_b200_mha_config* cfg,
                                                    const welvet_b200_kv8_cache* cache, int32_t seq,
                                                    const int32_t* seq_lens, int32_t max_ctx, const void* q,

@@ -10,12 +10,16 @@
 // to 128 rows, and a thread of the softmax holds one key of every column: no work is
 // spent on absent queries, and no row reductions across lanes are needed per tile.
 // What the small operands lose in 8 bits is kept in more of them:
-//   * a query row, scaled by a power of two to at most 448, is a sum of two E4M3 codes:
-//     exact to 2^-10 of 448, i.e. BF16 queries to 2^-19 of the row's largest value;
+//   * a query row, scaled by a power of two so that its largest value lies in (224, 448],
+//     is a sum of two E4M3 codes: a BF16 query has 8 bits, the codes 4 each, and only the
+//     smallest step of a code, 2^-9, cuts. Off by at most 2^-10, which is 2^-17 of the
+//     row's largest value;
 //   * a probability, rounded to FP16, is hi + lo/8 + lo2/64 in E5M2 codes (3 significant
 //     bits each, rounded to nearest in turn): a relative 2^-9 down to 2^-19 of the
 //     largest, and 2^-28 of the largest below that, so that long tails of small
-//     probabilities still add up. E4M3 codes would be finer but end at 2^-14.
+//     probabilities still add up. E4M3 codes would be finer but end at 2^-14. The row's
+//     sum takes the probabilities before this rounding, so a row that one key rules is off
+//     by up to 2^-9 as a whole, less than half a place of its BF16 output.
 // The codes of one sum are columns side by side (2 RT of S, 3 RT of O), added when
 // read: a 128-row MMA of 32 bytes takes about 60 cycles for any N up to 128, so one
 // wide MMA is cheaper than several narrow ones into the same columns.
@@ -39,13 +43,15 @@
 // are joined through distributed shared memory in rank order: no workspace, no second
 // launch, the same bits every time. An unsplit one goes from TMEM to the output.
 //
-// Measured. 32 sequences of 8192 tokens, 32 KV heads of 128: 305-320 us, 6.7-7.0 TB/s of
+// Measured, in a CUDA graph (calls on a stream take 3 to 4 % more). 32 sequences of 8192 tokens, 32 KV heads of 128: 305-320 us, 6.7-7.0 TB/s of
 // codes and scales; 64 of 4096, 8 KV heads of 64 for 32 heads: 46 us, 5.3 TB/s; 5 tokens
 // each for 8 sequences in a window of 8192, 8 KV heads of 128: 34-38 us, 3.6-4 TB/s (6.3
 // in the loop, the rest is the first tile's chain of lengths, page ids, copies, MMA and
 // softmax, and the joining); 2048 tokens over 10001, 32 heads of 128: 555 us, 543
-// TFLOP/s. The first three are bound by HBM; the last by the issue of the softmax, about
-// 300 instructions a warp and tile of 16 columns (the tensor pipe is 30 % busy).
+// TFLOP/s. The first three are bound by HBM; the last by the issue of the softmax in this
+// layout, about 300 instructions a warp and tile of 16 columns (the tensor pipe is 30 %
+// busy). The layout is for few query rows; a prompt piece has thousands a KV head, and
+// query rows as the 128-row operand over tiles widened to BF16 have not been tried.
 // Masked keys and rows past the context: their p is set to 0 and their V rows cleared
 // (a byte never written may be a NaN code); NaN scales reach only columns that see them.
 #include "attn_common.cuh"

@@ -200,11 +200,14 @@ __global__ void __launch_bounds__(1024) dgamma_kernel(const float* partial, int 
 // sit in one lane, and a warp keeps the angles of its token and the gammas of its side
 // in registers over all heads of its share. Bound by HBM: two groups of rows are
 // requested before the first is used. Forward: 16 bytes a load (16384 tokens x 64 heads
-// of 128, BF16: 92 us, 5.9 TB/s, 0.91 of the copy rate). Backward: four pairs a lane,
-// since x, dy, gamma, its gradient and the angles of eight pairs take 161 registers, 8
-// warps an SM: 143 us for 16384 x 40 heads of 128, against 104 (4.9 TB/s, 0.75 of the
-// copy rate); two chains of shuffles a row at 32 warps bound it, not loads on their way
-// (rows fetched three pieces ahead into shared memory: 101 to 131 us).
+// of 128, BF16: 92 us, 5.9 TB/s, 0.91 of the copy rate; x 40 heads, FP32: 108 us, 0.96;
+// in a CUDA graph, 95 a call). Backward: four pairs a lane, since x, dy, gamma, its
+// gradient and the angles of eight pairs take 161 registers, 8 warps an SM: 143 us for
+// 16384 x 40 heads of 128, against 103 (108 a call; 5.0 TB/s, 0.76 of the copy rate). What
+// keeps it there: a warp takes whole tokens over a fixed grid, so the busiest does 80 row
+// groups of a mean of 69 here (48 of 35 for 8192 tokens), and its loads are the leading
+// stall (5.3 warps an issue; shuffles 1.3), although rows fetched three pieces ahead into
+// shared memory took 101 to 131 us. Even shares of row groups have not been tried.
 template <class T, int HD, bool BWD> struct VT {
   static constexpr int VEC = BWD ? 4 : 16 / (int)sizeof(T), LPR = HD / 2 / VEC, RPW = 32 / LPR;
 };
