@@ -6,7 +6,7 @@ import pytest
 
 import welvet_b200 as W
 from conftest import rel_err
-from test_gpu_kv8 import _cache, _read
+from test_gpu_kv8 import _cache, _config, _read
 from test_gpu_kv8_layer import Ref, _gammas
 
 pytestmark = pytest.mark.gpu
@@ -179,3 +179,25 @@ def test_a_cut_block_keeps_its_scale(torch_cuda, hd):
     append(32, rows[:1])
     assert kscale[2] == 2.0 ** -6
     W.device_check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 96, 34])
+@pytest.mark.parametrize("window", [0, 40])
+def test_lengths_far_past_the_table_are_reported(torch_cuda, hd, window):
+    """A length that the block table cannot hold, up to the largest there is, ends with
+    code 4 and without a walk over its keys; other sequences are not touched by it."""
+    torch = torch_cuda
+    cache = _cache(torch, 3, [120] * 3, 2, hd)
+    cfg = _config(4, 2, hd, **(dict(mask=3, window=window) if window else {}))
+    q = torch.randn(3 * 2, 4 * hd, device="cuda").bfloat16()
+    good = torch.empty_like(q)
+    W.kv8_attention(cfg, cache, 2, q, good, 120)
+    W.device_check()
+    for wrong in (129, 1 << 20, (1 << 31) - 32, (1 << 31) - 1):
+        cache.tensors[5][1] = wrong
+        out = torch.empty_like(q)
+        W.kv8_attention(cfg, cache, 2, q, out, 120)
+        with pytest.raises(W.WelvetError) as e:
+            W.device_check()
+        assert e.value.code == 4 and "block table" in e.value.message
+        assert torch.equal(out[:2], good[:2]) and torch.equal(out[4:], good[4:])

@@ -289,11 +289,14 @@ __global__ void __launch_bounds__(kGenWarps * 32) kv8_attn_rows_kernel(const Kv8
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + row * a.ldq + (size_t)h * hd;
   for (int d = threadIdx.x; d < hd; d += blockDim.x) qs[d] = __bfloat162float(q[d]);
   __syncthreads();
-  const int k1 = qpos + 1, k0 = a.window > 0 ? max(0, k1 - a.window) : 0;
+  const int most = a.c.max_pages * kKv8Page;  // a length past the table is recorded and cut there
+  if (qpos >= most && threadIdx.x == 0 && a.err) atomicCAS(a.err, 0u, kErrKvPage);
+  const int k1 = min(qpos, most - 1) + 1, k0 = a.window > 0 ? max(0, qpos - a.window + 1) : 0;
   const float sl = a.scale * 1.4426950408889634f;
   const float slope = ALIBI ? exp2f(-(float)(a.head_base + h + 1) * 8.0f / (float)a.total_heads) * 1.4426950408889634f : 0.f;
   float m = -INFINITY, l = 0.f, o[kDims] = {};
-  for (int g = k0 / 32 + warp; g * 32 < k1; g += kGenWarps) {
+  const int groups = (k1 + 31) / 32;
+  for (int g = k0 / 32 + warp; g < groups; g += kGenWarps) {
     const int page = kv8_page(a.c, b, g * 32 / kKv8Page, a.err);
     if (page < 0) continue;
     const size_t ph = (size_t)page * a.c.kv_heads + kh;
