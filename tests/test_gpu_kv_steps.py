@@ -201,3 +201,24 @@ def test_lengths_far_past_the_table_are_reported(torch_cuda, hd, window):
             W.device_check()
         assert e.value.code == 4 and "block table" in e.value.message
         assert torch.equal(out[:2], good[:2]) and torch.equal(out[4:], good[4:])
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_prefill_refuses_the_cache_of_another_shape(torch_cuda, e4m3):
+    """The cache's layer says how its rows lie; decode takes no other layer's cache at all."""
+    torch = torch_cuda
+    layer = _layer(heads=4, kv=2, hd=64)
+    cache = W.KvCache(layer, 2, 64, e4m3=e4m3)
+    for other in (_layer(heads=4, kv=4, hd=64), _layer(heads=4, kv=2, hd=128), _layer(heads=4, kv=1, hd=64)):
+        x = torch.randn(2 * 8, 256, device="cuda").bfloat16()
+        with pytest.raises(W.WelvetError) as e:
+            other.prefill(cache, 2, 8, x, None, torch.empty_like(x))
+        assert e.value.code == 1
+    single = W.MhaLayer(W.MhaConfig.make(256, 4, 2, head_dim=64, precision=0, max_seq_len=512), *W.xavier_weights(256, 256, 128, 2))
+    x = torch.randn(2 * 8, 256, device="cuda")
+    with pytest.raises(W.WelvetError) as e:
+        single.prefill(cache, 2, 8, x, None, torch.empty_like(x))
+    assert e.value.code == 1
+    x = x.bfloat16()
+    layer.prefill(cache, 2, 8, x, None, torch.empty_like(x))
+    layer.check_device()

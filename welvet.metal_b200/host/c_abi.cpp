@@ -245,6 +245,9 @@ welvet_status welvet_b200_mha_prefill(welvet_b200_mha* layer, welvet_b200_kv* kv
     return wv::to_c(Status::err(1, "mha prefill: needs seq_mode 1 (per-sequence positions)"));
   if (batch > kv->kv->max_batch || seq > kv->kv->max_ctx)
     return wv::to_c(Status::err(1, "mha prefill: exceeds the KV cache"));
+  const wv::Mha *m = layer->m, *of = kv->kv->layer;  // the cache's rows are laid out by its own layer
+  if (m != of && (m->khc != of->khc || m->cfg.hd != of->cfg.hd || m->precision != of->precision || m->dev != of->dev))
+    return wv::to_c(Status::err(1, "mha prefill: the KV cache belongs to a layer of another shape, precision or device"));
   return wv::to_c(wv::mha_forward(layer->m, batch, seq, x, pre, post, on_device != 0, as_stream(stream), kv->kv));
 }
 
