@@ -306,7 +306,8 @@ WELVET_API welvet_status welvet_b200_decode_attention_static(const welvet_b200_m
  * pool its block unwritten and the attention rows that needed it unspecified.
  *
  * RoPE table: (cos, sin) of pos / theta^(2i/head_dim), [max_pos][head_dim/2][2] FP32,
- * computed in FP64, the table the layer uses (shaders/ops_mha.metal:14-29). */
+ * computed in FP64, the table the layer uses (shaders/ops_mha.metal:14-29). Tables are
+ * 8-byte aligned, everything else by its element (code 1 otherwise). */
 WELVET_API welvet_status welvet_b200_rope_table(int32_t max_pos, int32_t head_dim, double theta, float* table,
                                                 void* stream);
 

@@ -43,6 +43,12 @@ template <class F> welvet_status entry(const char* name, F&& body) {
   }
 }
 
+// Whether every pointer (null ones aside) is a multiple of n bytes: kernels load rows by
+// element at least, and a table's (cos, sin) together.
+template <class... P> bool aligned(size_t n, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % n == 0) && ...);
+}
+
 Status norm_args(const char* name, int64_t tokens, int heads, int kv_heads, int head_dim, double eps,
                  const float* q_gamma, const float* k_gamma, const float* rope, int max_pos, const int* positions,
                  int pos_mod, const void* q, int64_t ldq, const void* k, int64_t ldk, void* q_out, int64_t ldqo,
@@ -56,12 +62,12 @@ Status norm_args(const char* name, int64_t tokens, int heads, int kv_heads, int 
   const int64_t qd = (int64_t)heads * head_dim, kd = (int64_t)kv_heads * head_dim;
   if (tokens > 0 && ((heads && (!q || !q_out)) || (kv_heads && (!k || !k_out))))
     return Status::err(1, who + ": invalid argument");
+  if (!aligned(io_bf16 ? 2 : 4, q, k, q_out, k_out) || !aligned(4, q_gamma, k_gamma, positions) || !aligned(8, rope))
+    return Status::err(1, who + ": misaligned pointer");
   if ((heads && (ldq < qd || ldqo < qd)) || (kv_heads && (ldk < kd || ldko < kd)))
     return Status::err(1, who + ": row stride smaller than heads * head_dim");
   if (tokens > INT_MAX || tokens * (heads + (int64_t)kv_heads) > INT_MAX)
     return Status::err(1, who + ": tokens * heads too large");
-  DeviceCtx* d = nullptr;
-  WV_TRY(device_ctx(-1, &d));
   QkNormArgs& a = *out;
   a.tokens = tokens;
   a.heads = heads;
@@ -83,8 +89,15 @@ Status norm_args(const char* name, int64_t tokens, int heads, int kv_heads, int 
   a.k_out = k_out;
   a.ldqo = ldqo;
   a.ldko = ldko;
-  a.err = d->err;
-  a.sm_count = d->sm_count;
+  return Status::ok();
+}
+
+// The current device's part of the arguments, after the checks that need none.
+template <class Args> Status on_device(Args* a) {
+  DeviceCtx* d = nullptr;
+  WV_TRY(device_ctx(-1, &d));
+  a->err = d->err;
+  a->sm_count = d->sm_count;
   return Status::ok();
 }
 
@@ -97,6 +110,7 @@ Status cache_args(const char* name, const welvet_b200_kv8_cache* c, int seq, Kv8
     return Status::err(2, who + ": head_dim must be even and at most " + std::to_string(kKv8MaxHeadDim));
   if (c->batch > 65535 || c->kv_heads > 32767 || c->max_pages > INT_MAX / kKv8Page)
     return Status::err(1, who + ": batch, kv_heads or max_pages too large");
+  if (!aligned(4, c->k_scale, c->v_scale, c->block_table, c->ctx_len)) return Status::err(1, who + ": misaligned pointer");
   out->k = c->k;
   out->v = c->v;
   out->k_scale = c->k_scale;
@@ -119,6 +133,7 @@ welvet_status welvet_b200_rope_table(int32_t max_pos, int32_t head_dim, double t
   return wv::entry("rope_table", [&]() -> wv::Status {
     if (max_pos <= 0 || head_dim < 2 || head_dim % 2 || !(theta > 0) || !table)
       return wv::Status::err(1, "rope_table: invalid argument");
+    if (!wv::aligned(8, table)) return wv::Status::err(1, "rope_table: misaligned pointer");
     wv::DeviceCtx* d = nullptr;
     WV_TRY(wv::device_ctx(-1, &d));
     WV_CUDA(wv::rope_table(reinterpret_cast<float2*>(table), max_pos, head_dim, theta, static_cast<cudaStream_t>(stream)),
@@ -138,6 +153,7 @@ welvet_status welvet_b200_qk_norm_rope_forward(int64_t tokens, int32_t heads, in
     wv::QkNormArgs a;
     WV_TRY(wv::norm_args("qk_norm_rope", tokens, heads, kv_heads, head_dim, eps, q_gamma, k_gamma, rope, max_pos,
                          positions, pos_mod, q, ldq, k, ldk, q_out, ldq_out, k_out, ldk_out, io_bf16, &a));
+    WV_TRY(wv::on_device(&a));
     if (tokens == 0) return wv::Status::ok();
     WV_CUDA(wv::qk_norm_forward(a, static_cast<cudaStream_t>(stream)), "qk_norm_rope");
     wv::count_launch();
@@ -165,8 +181,11 @@ welvet_status welvet_b200_qk_norm_rope_backward(int64_t tokens, int32_t heads, i
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || (tokens > 0 && heads && !dq_out) ||
         (tokens > 0 && kv_heads && !dk_out) || (dq_gamma && !q_gamma) || (dk_gamma && !k_gamma))
       return wv::Status::err(1, std::string(name) + ": invalid argument");
+    if (!wv::aligned(io_bf16 ? 2 : 4, dq_out, dk_out) || !wv::aligned(4, dq_gamma, dk_gamma))
+      return wv::Status::err(1, std::string(name) + ": misaligned pointer");
     if ((heads && lddq_out < (int64_t)heads * head_dim) || (kv_heads && lddk_out < (int64_t)kv_heads * head_dim))
       return wv::Status::err(1, std::string(name) + ": row stride smaller than heads * head_dim");
+    WV_TRY(wv::on_device(&a));
     a.dq_out = dq_out;
     a.dk_out = dk_out;
     a.lddqo = lddq_out;
@@ -188,9 +207,10 @@ welvet_status welvet_b200_kv8_append(const welvet_b200_kv8_cache* cache, int32_t
     WV_TRY(wv::cache_args("kv8_append", cache, seq, &a.c));
     const int64_t row = (int64_t)cache->kv_heads * cache->head_dim;
     if (!k || !v || (rope && max_pos <= 0)) return wv::Status::err(1, "kv8_append: invalid argument");
+    if (!wv::aligned(2, k, v) || !wv::aligned(4, seq_lens) || !wv::aligned(8, rope))
+      return wv::Status::err(1, "kv8_append: misaligned pointer");
     if (ldk < row || ldv < row) return wv::Status::err(1, "kv8_append: row stride smaller than kv_heads * head_dim");
-    wv::DeviceCtx* d = nullptr;
-    WV_TRY(wv::device_ctx(-1, &d));
+    WV_TRY(wv::on_device(&a));
     a.batch = cache->batch;
     a.seq = seq;
     a.seq_lens = seq_lens;
@@ -200,8 +220,6 @@ welvet_status welvet_b200_kv8_append(const welvet_b200_kv8_cache* cache, int32_t
     a.ldv = ldv;
     a.rope = reinterpret_cast<const float2*>(rope);
     a.max_pos = max_pos;
-    a.err = d->err;
-    a.sm_count = d->sm_count;
     WV_CUDA(wv::kv8_append(a, static_cast<cudaStream_t>(stream)), "kv8_append");
     wv::count_launch();
     return wv::Status::ok();
@@ -215,6 +233,7 @@ welvet_status welvet_b200_kv8_attention(const welvet_b200_mha_config* cfg, const
     if (!cfg || !q || !out || max_ctx <= 0) return wv::Status::err(1, "kv8_attention: invalid argument");
     wv::Kv8AttnArgs a;
     WV_TRY(wv::cache_args("kv8_attention", cache, seq, &a.c));
+    if (!wv::aligned(2, q, out) || !wv::aligned(4, seq_lens)) return wv::Status::err(1, "kv8_attention: misaligned pointer");
     wv::Cfg c;
     WV_TRY(wv::resolve_config(*cfg, &c));
     a.heads = c.c.head_count;
