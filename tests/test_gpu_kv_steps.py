@@ -222,3 +222,28 @@ def test_prefill_refuses_the_cache_of_another_shape(torch_cuda, e4m3):
     x = x.bfloat16()
     layer.prefill(cache, 2, 8, x, None, torch.empty_like(x))
     layer.check_device()
+
+
+def test_lengths_are_read_before_the_call_returns(torch_cuda):
+    """A page-locked array that changes right behind the call, the stream still busy."""
+    torch = torch_cuda
+    layer = _layer()
+    x0, x = torch.randn(2 * 40, 256, device="cuda").bfloat16(), torch.randn(2, 256, device="cuda").bfloat16()
+    big = torch.randn(8192, 8192, device="cuda").bfloat16()
+    got = []
+    for pinned in (False, True):
+        cache = W.KvCache(layer, 2, 64)
+        layer.prefill(cache, 2, 40, x0, None, torch.empty_like(x0))
+        if pinned:
+            lengths = torch.tensor([30, 11], dtype=torch.int32).pin_memory()
+            for _ in range(20):
+                big @ big
+            W.check(W.lib().welvet_b200_kv_set_lengths(cache.handle, 2, lengths.data_ptr(), None))
+            lengths.fill_(3)
+        else:
+            cache.set_lengths([30, 11])
+        pre, post = torch.empty(2, 256, device="cuda", dtype=torch.bfloat16), torch.empty_like(x)
+        layer.decode(cache, 2, x, pre, post)
+        layer.check_device()
+        got.append(pre)
+    assert torch.equal(*got)

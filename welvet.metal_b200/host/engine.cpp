@@ -1289,9 +1289,12 @@ Status kv_set_lengths(Kv* kv, int batch, const int* lengths, cudaStream_t s) {
     if (lengths[b] < 0 || lengths[b] > kv->max_ctx) return Status::err(1, "kv lengths: outside 0 ... max_ctx");
   std::lock_guard<std::mutex> lock(kv->layer->mu);
   WV_CUDA(cudaSetDevice(kv->layer->dev->device), "cudaSetDevice");
-  // pageable host memory: the copy has read it when the call returns
-  WV_CUDA(cudaMemcpyAsync(kv->ctx_len.p, lengths, (size_t)batch * 4, cudaMemcpyHostToDevice, s), "kv lengths");
-  for (int b = 0; b < batch; ++b) kv->ctx_host[b] = lengths[b];
+  // From a copy in pageable memory, which the transfer has read when it returns; the
+  // caller's array may be page-locked, and that would be read when the stream gets there.
+  std::vector<int> now(kv->ctx_host);
+  std::copy(lengths, lengths + batch, now.begin());
+  WV_CUDA(cudaMemcpyAsync(kv->ctx_len.p, now.data(), (size_t)batch * 4, cudaMemcpyHostToDevice, s), "kv lengths");
+  kv->ctx_host.swap(now);
   return Status::ok();
 }
 
